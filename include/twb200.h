@@ -208,6 +208,18 @@ int tw_rope_heads(const void* x, void* y, long long tokens, int heads, long long
                   float eps, void* stream);
 /* x[r, :] = bf16(x[r, :] + gate[r / rows_per_batch, :] * y[r, :]) in place (gated residual of a DiT block). */
 int tw_gate_residual(void* x, const void* gate, const void* y, int rows, int hidden, int rows_per_batch, void* stream);
+/* The gated residual with the norm after the block and the norm before the next one, one pass:
+ *   z = y, or with post_norm y * rsqrt(mean(y^2) + eps) [* post_weight] per row (not rounded);
+ *   x[r, :] = bf16(residual_scale * x[r, :] + gate[b, :] * z) in place (gate NULL: ones);
+ *   h[r, :] = what tw_rms_norm gives for the new x with weight, shift, scale; stats as there.
+ * Without post_norm and with residual_scale = 1 the bits are those of tw_gate_residual followed by tw_rms_norm.
+ * x, y, h must not overlap. hidden % 8 == 0, hidden <= 16384. */
+int tw_gate_residual_norm(void* x, const void* y, const void* gate, const void* post_weight, int post_norm, float residual_scale,
+                          const void* weight, const void* shift, const void* scale, void* h, float* stats, void* scratch,
+                          int rows, int hidden, int rows_per_batch, float eps, void* stream);
+/* Id of the stream capture that `stream` is part of, 0 when it is not capturing. Host function: a caller that keeps a
+ * scratch per stream uses it to keep one per captured graph as well. */
+unsigned long long tw_capture_id(void* stream);
 
 #ifdef __cplusplus
 }

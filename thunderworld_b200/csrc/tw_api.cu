@@ -21,6 +21,13 @@ extern "C" const char* tw_status(int status) {
 
 extern "C" int tw_abi_version(void) { return 3; }
 
+extern "C" unsigned long long tw_capture_id(void* stream) {
+  cudaStreamCaptureStatus state = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &state, &id) != cudaSuccess) { (void)cudaGetLastError(); return 0; }
+  return state == cudaStreamCaptureStatusActive ? id : 0;
+}
+
 // ---------------------------------------------------------------------------------------------
 // Self-test of the bounded-wait protocol every kernel of this library uses: one warp waits on a barrier
 // nobody ever arrives at, gives up after `limit_cycles`, and the status word reports it. Nothing is in

@@ -11,6 +11,8 @@
 //   tw_rope_heads     exact-rounding rotary embedding of such rows (cosmos/pipeline_tuning.py:42-63), optionally
 //                     after the head norm in the same pass
 //   tw_gate_residual  x += gate[b] * y
+//   tw_gate_residual_norm  the gated residual together with the norm after the block (on y) and the norm before the
+//                     next one (on the new x): what lies between two projections of a block, in one pass
 //
 // All are HBM-bound: 16-byte loads and stores, every input element read once. The factor is finished by the
 // last CTA to retire (ticket counter in an 8-byte scratch that the kernel leaves zeroed), so no second launch
@@ -260,6 +262,117 @@ __global__ void __launch_bounds__(256) gate_residual_kernel(uint4* __restrict__ 
   }
 }
 
+// ---- gated residual with the norms around it ------------------------------------------------------
+// z = y, or y * rsqrt(mean(y^2) + eps) [* post_weight] (POST: the norm after the block);
+// x' = bf16(residual_scale * x + gate * z);  h = bf16(x' * rsqrt(mean(x'^2) + eps) [* weight] [* (1 + scale) + shift]).
+// One CTA per row; a row of x and y is read once, x' stays in registers between the two norms, so a pass moves
+// 8 bytes per element where gate_residual and rms_norm one after the other move 10. x' is rounded before it is
+// squared, because the next block reads the rounded stream; z is not rounded on its own. The sums of squares are
+// held in 32 bits and taken in rms_norm_kernel's order, so that without POST and with residual_scale = 1 the bits
+// are those of the two kernels.
+// Sum over the 256 threads of a block in rms_norm_kernel's order.
+__device__ __forceinline__ float block_sum_256(float v, float* part) {
+  v = warp_sum(v);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return part[0] + part[1] + part[2] + part[3] + part[4] + part[5] + part[6] + part[7];
+}
+
+template <int VPT, bool POST>   // 16-byte vectors per thread, 256 threads
+__global__ void __launch_bounds__(256) gate_residual_norm_kernel(uint4* __restrict__ x, const uint4* __restrict__ y,
+                                                                 const uint4* __restrict__ gate, const uint4* __restrict__ post_weight,
+                                                                 const uint4* __restrict__ weight, const uint4* __restrict__ shift,
+                                                                 const uint4* __restrict__ scale, uint4* __restrict__ h,
+                                                                 int hidden_vecs, int rows_per_batch, float residual_scale,
+                                                                 float eps, unsigned* scratch, float* stats) {
+  __shared__ float post_part[8], part[8];
+  const int row = blockIdx.x;
+  const size_t base = (size_t)row * hidden_vecs, mod = (size_t)(row / rows_per_batch) * hidden_vecs;
+  uint4 xv[VPT], yv[VPT];
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int c = threadIdx.x + j * 256;
+    if (c < hidden_vecs) { yv[j] = __ldg(y + base + c); xv[j] = x[base + c]; }
+  }
+  float post_rstd = 1.f;
+  if (POST) {
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      if (threadIdx.x + j * 256 < hidden_vecs) {
+        float b[8];
+        unpack8(yv[j], b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = __fmaf_rn(b[i], b[i], ss);
+      }
+    }
+    post_rstd = rsqrtf(block_sum_256(ss, post_part) / (float)(hidden_vecs * 8) + eps);
+  }
+  float ss = 0.f, unused = 0.f;
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int c = threadIdx.x + j * 256;
+    if (c < hidden_vecs) {
+      float a[8], b[8];
+      unpack8(xv[j], a);
+      unpack8(yv[j], b);
+      if (POST) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] *= post_rstd;
+        if (post_weight) {
+          float w[8];
+          unpack8(__ldg(post_weight + c), w);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) b[i] *= w[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] *= residual_scale;          // exact when the scale is 1
+      if (gate) {
+        float g[8];
+        unpack8(__ldg(gate + mod + c), g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[i] = __fmaf_rn(g[i], b[i], a[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[i] += b[i];
+      }
+      xv[j] = pack8(a, unused);
+      x[base + c] = xv[j];
+      unpack8(xv[j], a);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = __fmaf_rn(a[i], a[i], ss);
+    }
+  }
+  const float rstd = rsqrtf(block_sum_256(ss, part) / (float)(hidden_vecs * 8) + eps);
+  float peak = 0.f;
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int c = threadIdx.x + j * 256;
+    if (c < hidden_vecs) {
+      float r[8];
+      unpack8(xv[j], r);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] *= rstd;
+      if (weight) {
+        float w[8];
+        unpack8(__ldg(weight + c), w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] *= w[i];
+      }
+      if (scale) {
+        float sc[8], sh[8];
+        unpack8(__ldg(scale + mod + c), sc);
+        unpack8(__ldg(shift + mod + c), sh);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = __fmaf_rn(r[i], 1.f + sc[i], sh[i]);
+      }
+      h[base + c] = pack8(r, peak);
+    }
+  }
+  if (stats) finish_factor(peak, scratch, stats);
+}
+
 int grid_for(long long vecs) {
   const long long want = (vecs + 255) / 256;
   return (int)(want < 148 * 16 ? (want > 0 ? want : 1) : 148 * 16);
@@ -348,5 +461,39 @@ extern "C" int tw_gate_residual(void* x, const void* gate, const void* y, int ro
   const long long vecs = (long long)rows * (hidden / 8);
   gate_residual_kernel<<<grid_for(vecs), 256, 0, static_cast<cudaStream_t>(stream_)>>>(
       static_cast<uint4*>(x), static_cast<const uint4*>(gate), static_cast<const uint4*>(y), vecs, hidden / 8, rows_per_batch);
+  return cudaGetLastError() == cudaSuccess ? TW_OK : TW_ERR_LAUNCH;
+}
+
+extern "C" int tw_gate_residual_norm(void* x, const void* y, const void* gate, const void* post_weight, int post_norm,
+                                     float residual_scale, const void* weight, const void* shift, const void* scale, void* h,
+                                     float* stats, void* scratch, int rows, int hidden, int rows_per_batch, float eps,
+                                     void* stream_) {
+  if (!x || !y || !h || rows <= 0 || hidden <= 0 || rows_per_batch <= 0 || (stats && !scratch) || (!shift != !scale) ||
+      (post_weight && !post_norm))
+    return TW_ERR_ARGUMENT;
+  if (hidden % 8) return TW_ERR_SHAPE;
+  if (hidden > 8 * 256 * 8) return TW_ERR_TOO_LARGE;
+  if (misaligned(x) || misaligned(y) || misaligned(h) || misaligned(gate) || misaligned(post_weight) || misaligned(weight) ||
+      misaligned(shift) || misaligned(scale))
+    return TW_ERR_ALIGNMENT;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  const int hv = hidden / 8, vpt = (hv + 255) / 256;
+  auto launch = [&](auto kernel) {
+    kernel<<<rows, 256, 0, stream>>>(static_cast<uint4*>(x), static_cast<const uint4*>(y), static_cast<const uint4*>(gate),
+                                     static_cast<const uint4*>(post_weight), static_cast<const uint4*>(weight),
+                                     static_cast<const uint4*>(shift), static_cast<const uint4*>(scale), static_cast<uint4*>(h),
+                                     hv, rows_per_batch, residual_scale, eps, static_cast<unsigned*>(scratch), stats);
+  };
+  if (post_norm) {
+    if (vpt <= 1) launch(gate_residual_norm_kernel<1, true>);
+    else if (vpt <= 2) launch(gate_residual_norm_kernel<2, true>);
+    else if (vpt <= 4) launch(gate_residual_norm_kernel<4, true>);
+    else launch(gate_residual_norm_kernel<8, true>);
+  } else {
+    if (vpt <= 1) launch(gate_residual_norm_kernel<1, false>);
+    else if (vpt <= 2) launch(gate_residual_norm_kernel<2, false>);
+    else if (vpt <= 4) launch(gate_residual_norm_kernel<4, false>);
+    else launch(gate_residual_norm_kernel<8, false>);
+  }
   return cudaGetLastError() == cudaSuccess ? TW_OK : TW_ERR_LAUNCH;
 }

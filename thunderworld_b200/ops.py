@@ -10,6 +10,7 @@ Host-side mirror of the reference's packers and launch wrappers:
 torch is used for device memory and streams only.
 """
 import ctypes
+from contextlib import nullcontext
 from dataclasses import dataclass
 import torch
 from . import _lib
@@ -313,6 +314,79 @@ def rope_heads(x, cos, sin, *, norm=False, eps=1e-6):
                                          _ptr(sin), cos.shape[0], int(cos.dtype == torch.bfloat16), int(norm), float(eps),
                                          _stream(x.device)))
     return y
+
+
+# Scratch that a kernel leaves zeroed, one per stream: calls on one stream run one after the other. A call that is being
+# captured gets one of its own graph (zeroed by the graph on every replay), so that two graphs captured on one stream may
+# be replayed side by side; only the newest capture's is held here, older ones live as long as their graph's pool.
+_stream_scratch = {}
+
+
+def _scratch(device, stream):
+    capture = _lib.load().tw_capture_id(stream)
+    key = (device, stream, capture != 0)
+    held = _stream_scratch.get(key)
+    if held is None or held[0] != capture:
+        held = _stream_scratch[key] = (capture, torch.zeros(8, device=device, dtype=torch.uint8))
+    return held[1]
+
+
+_same_device = nullcontext()
+
+
+def _device(device):
+    """Context that makes `device` current; nothing to do, and nothing done, when it is."""
+    return _same_device if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _overlap(a, b):
+    """Whether two contiguous tensors share memory."""
+    return a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
+
+
+def gate_residual_norm_(x, y, gate=None, *, post_norm=False, post_weight=None, residual_scale=1., weight=None, shift=None,
+                        scale=None, eps=1e-6, want_factor=False, return_stats=False):
+    """The gated residual and the norm that follows it in one pass: x = residual_scale * x + gate[:, None, :] * z in place,
+    where z is y, or with post_norm (implied by post_weight) the RMSNorm of y times post_weight; returns
+    rms_norm(x, weight, eps, shift=shift, scale=scale, ...) of the new x, with want_factor / return_stats as there.
+    x, y [batch, tokens, hidden]; gate, shift, scale [batch, hidden]; gate None: ones. Without post_norm and with
+    residual_scale 1 the bits are those of gate_residual_ followed by rms_norm."""
+    given = [t for t in (x, y, gate, post_weight, weight, shift, scale) if t is not None]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+        raise RuntimeError('Fused residual and norm requires inference mode')
+    _check_bf16(*given)
+    dev, hidden = x.device, x.shape[-1]
+    if any(t.device != dev for t in given):
+        raise ValueError('all operands must be on one device')
+    if y.shape != x.shape:
+        raise ValueError('x and y must have equal shapes')
+    if not x.numel():
+        raise ValueError('empty residual streams are unsupported')
+    if any(t is not None and t.numel() != hidden for t in (weight, post_weight)):
+        raise ValueError('norm weights must be [hidden]')
+    if (shift is None) != (scale is None):
+        raise ValueError('shift and scale come together')
+    rows = per_batch = x.numel() // hidden
+    batched = [t for t in (gate, shift, scale) if t is not None]
+    if batched:
+        batch = batched[0].numel() // hidden
+        if any(t.shape[-1] != hidden or t.numel() != batch * hidden for t in batched) or not batch or rows % batch:
+            raise ValueError('gate, shift and scale must be [batch, hidden] with batch dividing the rows of x')
+        per_batch = rows // batch
+    if _overlap(x, y):
+        raise ValueError('x is updated in place and must not share memory with y')
+    require_sm100(dev)
+    h = torch.empty_like(x)
+    stats = torch.empty(2, device=dev, dtype=torch.float32) if want_factor else None
+    with _device(dev):
+        stream = _stream(dev)
+        _lib.check(_lib.load().tw_gate_residual_norm(
+            _ptr(x), _ptr(y), _ptr(gate), _ptr(post_weight), int(post_norm or post_weight is not None), float(residual_scale),
+            _ptr(weight), _ptr(shift), _ptr(scale), _ptr(h), _ptr(stats), _ptr(_scratch(dev, stream)) if want_factor else None,
+            rows, hidden, per_batch, float(eps), stream))
+    if not want_factor:
+        return h
+    return (h, stats) if return_stats else (h, stats[0])
 
 
 def gate_residual_(x, gate, y):
