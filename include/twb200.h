@@ -130,6 +130,27 @@ int tw_fused(int m, int n, int k, const void* a_codes, const void* w_codes, cons
  * 128). Pure host function. */
 int tw_fused_tile_n(int n);
 
+/* ---- products of a few rows ------------------------------------------------------------------
+ * out[r, n] = rnd( factor * sum_k bf16(x[r, k] * prescale[k]) * W[n, k] + bias[n] ), 1 <= r <= 32: the packed weights of
+ * tw_fused for a token at a time. x stays bf16 (no activation planes), sums are 32 bits wide, one rounding at the end.
+ * W[n, k] = code * scale (scale per 16 k), plus the bank's tile where (n / 128, k / 128) has one; bank layout, CSR, shared and
+ * dense as in TwRepairIO, every (n / 128, k / 128) at most once. Any n; k % 32 == 0, k <= 32768; with a bank n and k multiples of 128.
+ * Entries of off / wi / wloc that lead outside wi, K or the bank are left out. */
+typedef struct TwMatvecArgs {
+  const void* x;            /* bf16, row r at x + r * x_stride, 16-byte aligned rows */
+  long long x_stride;       /* elements, a multiple of 8 */
+  const float* prescale;    /* [k] or NULL */
+  const uint8_t *codes, *scales;   /* [n, k/2], [n, k/16] row-major E4M3 */
+  const float* factor;      /* device scalar */
+  const void* bias;         /* bf16 [n] or NULL */
+  const uint8_t *wr, *wrs;  /* bank codes [slots, 128, 64] / scales [slots, 128, 8], or NULL */
+  const int32_t *wi, *off, *wloc;
+  void* out;                /* [rows, n] contiguous */
+  int32_t rows, n, k, slots, entries, shared, dense; /* slots: tiles in the bank, 0: none; entries: length of wi (and wloc) */
+  int32_t out_f32;          /* 0: bf16, else float32 */
+} TwMatvecArgs;
+int tw_matvec(const TwMatvecArgs* args, void* stream);
+
 /* ---- streaming FP4 attention -----------------------------------------------------------------
  * Three calls replace the reference's attention launch chain (thunderworld_fp4/runtime.py:32-108):
  *   tw_pack_rows     pack_qk / pack_v        (_kernels.py:12-47): per-row factor max/1536, base + residual

@@ -1,0 +1,275 @@
+"""Products of a few rows with packed NVFP4 weights (`ops.fp4_matvec`) against their definition in 64 bits.
+
+Tolerances: the products are exact, the result is rounded once to bf16 (half a step: 2^-8 of the value; float32: 2^-24). A
+32-bit sum is added to at most K / 128 times by an instruction that itself adds 16 products, then 8 warps and up to 8 CTAs
+are added: each of these is off by at most 2^-22 (truncation inside the instruction counted as two steps) of the sum of the
+products' sizes S, so by (K / 128 + 32) 2^-22 S in all, factor and bias included in S."""
+import pytest
+import torch
+
+gpu = pytest.mark.gpu
+E2M1 = [0., .5, 1., 1.5, 2., 3., 4., 6.]
+
+
+def decoded(codes, scales):
+    lut = torch.tensor(E2M1 + [-v for v in E2M1], dtype=torch.float64, device=codes.device)
+    pairs = torch.stack([codes & 15, codes >> 4], -1).flatten(-2).long()
+    return lut[pairs] * scales.double().repeat_interleave(16, -1)
+
+
+def weights(n, k, seed, low=.01, high=448.):
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.uint8)
+    scales = (torch.rand((n, k // 16), generator=g) * (high - low) + low).to(torch.float8_e4m3fn)
+    scales.view(torch.uint8)[torch.rand((n, k // 16), generator=g) < .1] = 0          # groups of zeros
+    scales.view(torch.uint8)[torch.rand((n, k // 16), generator=g) < .05] = 1         # the smallest scale, 2^-9
+    return codes.cuda(), scales.cuda()
+
+
+def rows_of(r, k, seed):
+    return torch.randn(r, k, generator=torch.Generator().manual_seed(seed)).bfloat16().cuda()
+
+
+def bank_of(n, k, share, seed, shared=False):
+    g = torch.Generator().manual_seed(seed)
+    nb, kb = n // 128, k // 128
+    picked = torch.randperm(nb * kb, generator=g)[:max(1, round(share * nb * kb))].sort().values
+    off = torch.zeros(nb + 1, dtype=torch.int32)
+    off[1:] = torch.bincount(picked // kb, minlength=nb).cumsum(0)
+    slots = len(picked)
+    wr, wrs = weights(slots * 128, 128, seed + 1, high=30.)
+    wr, wrs = wr.view(slots, 128, 64), wrs.view(slots, 128, 8)
+    w1 = torch.zeros(n, k, dtype=torch.float64, device='cuda')
+    values = decoded(wr, wrs)
+    order = torch.randperm(slots, generator=g) if shared else torch.arange(slots)
+    for i, t in enumerate(picked.tolist()):
+        b, c = divmod(t, kb)
+        w1[b * 128:(b + 1) * 128, c * 128:(c + 1) * 128] = values[order[i]]
+    kw = dict(wr=wr, wrs=wrs, wi=(picked % kb).int().cuda(), off=off.cuda())
+    if shared:
+        kw.update(wloc=order.int().cuda(), shared=True)
+    return kw, w1
+
+
+def check(y, x, w, factor, bias=None, k=None):
+    x, k = x.double(), x.shape[-1]
+    want = (x @ w.T) * factor.double()
+    size = (x.abs() @ w.abs().T) * factor.double().abs()
+    if bias is not None:
+        want, size = want + bias.double(), size + bias.double().abs()
+    half = 2. ** -8 if y.dtype == torch.bfloat16 else 2. ** -24
+    bound = half * want.abs() + (k / 128 + 32) * 2. ** -22 * size
+    off = (y.double() - want).abs()
+    assert (off <= bound).all(), float((off - bound).max())
+
+
+SHAPES = [(1, 1, 32), (1, 16, 64), (3, 17, 96), (8, 100, 1024), (9, 257, 2080), (16, 2048, 2048), (17, 1000, 4096), (32, 130, 160),
+          (1, 5001, 4096), (2, 48, 32768), (32, 33, 24576), (31, 2049, 1120), (5, 128, 24576)]
+
+
+@gpu
+@pytest.mark.parametrize('r,n,k', SHAPES)
+@pytest.mark.parametrize('prescale,bias,out', [(False, False, torch.bfloat16), (True, True, torch.float32)])
+def test_definition(r, n, k, prescale, bias, out):
+    from thunderworld_b200 import ops
+    codes, scales = weights(n, k, n + k)
+    x = rows_of(r, k, r)
+    g = torch.Generator().manual_seed(4)
+    d = (torch.rand(k, generator=g) + .5).cuda() if prescale else None
+    b = torch.randn(n, generator=g).bfloat16().cuda() if bias else None
+    factor = torch.tensor(3e-4, device='cuda')
+    y = ops.fp4_matvec(x, codes, scales, factor, prescale=d, bias=b, out_dtype=out)
+    assert y.shape == (r, n) and y.dtype == out
+    held = x if d is None else (x.float() * d).bfloat16()
+    check(y, held, decoded(codes, scales), factor, b)
+    assert torch.equal(y, ops.fp4_matvec(x, codes, scales, factor, prescale=d, bias=b, out_dtype=out))     # a fixed order
+
+
+@gpu
+@pytest.mark.parametrize('r,n,k', [(1, 128, 128), (3, 256, 2048), (8, 2048, 8192), (20, 384, 24576), (2, 8192, 640)])
+@pytest.mark.parametrize('share,shared', [(.02, False), (.3, True), (1., False)])
+def test_bank(r, n, k, share, shared):
+    from thunderworld_b200 import ops
+    codes, scales = weights(n, k, 5)
+    bank, w1 = bank_of(n, k, share, 6, shared)
+    x, factor = rows_of(r, k, 7), torch.tensor([1e-3], device='cuda')
+    w = decoded(codes, scales) + w1
+    check(ops.fp4_matvec(x, codes, scales, factor, **bank), x, w, factor)
+    if share == 1.:                                     # every tile there: the dense form needs no lists
+        y = ops.fp4_matvec(x, codes, scales, factor, wr=bank['wr'], wrs=bank['wrs'], dense=True)
+        assert torch.equal(y, ops.fp4_matvec(x, codes, scales, factor, **bank))
+
+
+@gpu
+def test_bank_entries_that_lead_outside_are_left_out():
+    from thunderworld_b200 import ops
+    n, k = 256, 1024
+    codes, scales = weights(n, k, 5)
+    bank, w1 = bank_of(n, k, .5, 6, True)
+    x, factor = rows_of(4, k, 7), torch.tensor(1e-3, device='cuda')
+    bank['wi'][0], bank['wloc'][1], bank['wloc'][2] = 8, -1, len(bank['wr'])      # K block 8 of 8; no such bank position, twice
+    off = bank['off'].tolist()
+    bank['off'][2] += 1000                                                        # past the end of wi
+    full, _ = bank_of(n, k, .5, 6, True)
+    w1 = w1.clone()
+    for i in range(3):
+        b = 0 if i < off[1] else 1
+        c = int(full['wi'][i])
+        w1[b * 128:(b + 1) * 128, c * 128:(c + 1) * 128] = 0
+    check(ops.fp4_matvec(x, codes, scales, factor, **bank), x, decoded(codes, scales) + w1, factor)
+
+
+@gpu
+@pytest.mark.parametrize('size', [1e-38, 1e-30, 1e-6, 1e6, 1e30])
+def test_range_of_the_rows(size):
+    """bf16 has exponents that f16 does not: rows of every size, an outlier far above the rest, zeros."""
+    from thunderworld_b200 import ops
+    codes, scales = weights(64, 512, 1, high=4.)
+    factor = torch.tensor(1., device='cuda')
+    x = (rows_of(6, 512, 2).double() * size).bfloat16()
+    x[1] = 0
+    x[2, 17] = x[2].float().abs().max().double().item() * 2. ** 12 if size < 1e25 else x[2, 17]
+    x[3, :256] = 0
+    check(ops.fp4_matvec(x, codes, scales, factor, out_dtype=torch.float32), x, decoded(codes, scales), factor)
+
+
+@gpu
+def test_values_far_below_an_outlier_that_meets_zeros():
+    """The outlier's weights are zero, so what remains is the sum of values 2^20 below it: still exact, as 2^29 are held."""
+    from thunderworld_b200 import ops
+    codes, scales = weights(40, 256, 1, high=4.)
+    scales.view(torch.uint8)[:, 0] = 0
+    x = rows_of(2, 256, 3)
+    x[:, 5] = 2. ** 20
+    factor = torch.tensor(1., device='cuda')
+    w = decoded(codes, scales)
+    y = ops.fp4_matvec(x, codes, scales, factor, out_dtype=torch.float32)
+    x[:, 5] = 0
+    check(y, x, w, factor)
+
+
+@gpu
+def test_infinities_and_nan_stay_in_their_row():
+    from thunderworld_b200 import ops
+    codes, scales = weights(96, 256, 1)
+    codes |= 0x11                                                        # no zero codes
+    scales.view(torch.uint8)[scales.view(torch.uint8) == 0] = 8
+    x = rows_of(12, 256, 3)
+    x[2, 9], x[5, 200], x[9, 1] = float('inf'), float('nan'), float('-inf')
+    y = ops.fp4_matvec(x, codes, scales, torch.tensor(1e-3, device='cuda')).float()
+    w = decoded(codes, scales)
+    clean = [i for i in range(12) if i not in (2, 5, 9)]
+    assert torch.isfinite(y[clean]).all() and torch.isnan(y[5]).all()
+    assert torch.equal(y[2], torch.where(w[:, 9] > 0, torch.inf, -torch.inf).float())
+    assert torch.equal(y[9], torch.where(w[:, 1] > 0, -torch.inf, torch.inf).float())
+
+
+@gpu
+def test_views_streams_graphs_and_out():
+    from thunderworld_b200 import ops
+    codes, scales = weights(500, 1024, 1)
+    factor = torch.tensor(1e-3, device='cuda')
+    wide = rows_of(6, 3 * 1024, 2)
+    x = wide[::2, 1024:2048]                                              # strided rows
+    want = ops.fp4_matvec(x.contiguous(), codes, scales, factor)
+    assert torch.equal(ops.fp4_matvec(x, codes, scales, factor), want)
+    odd = torch.zeros(3 * 1024 + 1, device='cuda', dtype=torch.bfloat16)[1:].view(3, 1024)   # rows that no 16-byte load can take
+    odd.copy_(x)
+    assert torch.equal(ops.fp4_matvec(odd, codes, scales, factor), want)
+    assert torch.equal(ops.fp4_matvec(x[1], codes, scales, factor), want[1])
+    assert torch.equal(ops.fp4_matvec(x.contiguous().view(1, 3, 1024), codes, scales, factor), want[None])
+    out = torch.full((3, 500), 7., device='cuda', dtype=torch.bfloat16)
+    assert ops.fp4_matvec(x, codes, scales, factor, out=out) is out and torch.equal(out, want)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):                                                   # two calls at once: no shared workspace
+        for s in (a, b):
+            with torch.cuda.stream(s):
+                got.append(ops.fp4_matvec(x, codes, scales, factor))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y in got)
+    xs = x.contiguous()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.fp4_matvec(xs, codes, scales, factor)
+    xs.mul_(2)
+    graph.replay()
+    assert torch.equal(y, ops.fp4_matvec(xs, codes, scales, factor)) and not torch.equal(y, want)
+
+
+@gpu
+def test_offsets_past_32_bits():
+    """Codes of more than 4 GiB: rows at the end are read where they lie."""
+    from thunderworld_b200 import ops
+    n, k = 270001, 32768
+    codes = torch.zeros((n, k // 2), device='cuda', dtype=torch.uint8)
+    scales = torch.zeros((n, k // 16), device='cuda', dtype=torch.float8_e4m3fn)
+    at = [0, 131071, 131073, 262145, n - 1]
+    c, s = weights(len(at), k, 3)
+    codes[at], scales.view(torch.uint8)[at] = c, s.view(torch.uint8)
+    x, factor = rows_of(2, k, 1), torch.tensor(1e-3, device='cuda')
+    y = ops.fp4_matvec(x, codes, scales, factor)
+    check(y[:, at], x, decoded(c, s), factor)
+    y[:, at] = 0
+    assert not y.any()
+
+
+@gpu
+def test_modules():
+    """FP4Linear.matvec and Native.matvec multiply with the weights of their forward()."""
+    from thunderworld_b200 import FP4Linear, Native
+    from thunderworld_b200.native import quantize_weight
+    g = torch.Generator().manual_seed(1)
+    n, k = 384, 512
+    w = (torch.randn(n, k, generator=g) * .05).bfloat16().cuda()
+    d, bias = (torch.rand(k, generator=g) + .5).cuda(), torch.randn(n, generator=g).bfloat16().cuda()
+    layer = FP4Linear.from_float(w, prescale=d, bias=bias)
+    x = rows_of(5, k, 2)
+    check(layer.matvec(x), (x.float() * d).bfloat16(), decoded(layer.weight_codes, layer.weight_scales), layer.weight_global_scale, layer.bias)
+    codes, scales, wg = quantize_weight(w)
+    tiles = torch.rand(3, 4, generator=g) < .5
+    tiles[0, 0], tiles[1, 1] = True, False
+    wm = tiles.repeat_interleave(128, 0).repeat_interleave(128, 1).cuda()
+    op = Native(codes, scales, wg, torch.ones(k, device='cuda'), torch.ones(1, k, dtype=torch.bool, device='cuda'), wm)
+    both = decoded(codes[0], scales[0]) + decoded(codes[1], scales[1]) * wm
+    check(op.matvec(x, bias=bias), x, both, wg, bias)
+
+
+@gpu
+def test_refusals():
+    from thunderworld_b200 import ops
+    codes, scales = weights(128, 128, 1)
+    x, f = rows_of(4, 128, 2), torch.tensor(1., device='cuda')
+    call = ops.fp4_matvec
+    for bad, match in ((dict(x=x.float()), 'BF16'), (dict(x=x.cpu()), 'CUDA'), (dict(x=x[:, :64]), 'values per row'), (dict(x=x[:0]), 'empty'),
+                       (dict(x=rows_of(33, 128, 1)), 'at most 32'), (dict(codes=codes.view(-1, 32)), 'values per row'),
+                       (dict(codes=codes.int()), 'codes'), (dict(scales=scales[:, :4]), 'scales'), (dict(scales=scales.float()), 'scales'),
+                       (dict(factor=f.double()), 'factor'), (dict(prescale=torch.ones(64, device='cuda')), 'prescale'),
+                       (dict(bias=torch.ones(128, device='cuda')), 'bias'), (dict(out_dtype=torch.float16), 'out_dtype'),
+                       (dict(out=torch.empty(4, 64, device='cuda', dtype=torch.bfloat16)), 'out must'),
+                       (dict(factor=torch.tensor(1.)), 'share a CUDA device'), (dict(wr=codes.view(1, 128, 64)), 'wrs'),
+                       (dict(wr=codes.view(1, 128, 64), wrs=scales.view(1, 128, 8)), 'wi'),
+                       (dict(wr=codes.view(1, 128, 64), wrs=scales.view(1, 128, 8), wi=torch.zeros(1, dtype=torch.int32, device='cuda'),
+                             off=torch.zeros(3, dtype=torch.int32, device='cuda')), 'off')):
+        args = dict(x=x, codes=codes, scales=scales, factor=f) | bad
+        with pytest.raises(ValueError, match=match):
+            call(args.pop('x'), args.pop('codes'), args.pop('scales'), args.pop('factor'), **args)
+    with pytest.raises(RuntimeError, match='inference'):
+        call(x.clone().requires_grad_(), codes, scales, f)
+    with pytest.raises(RuntimeError, match='shape'):
+        call(rows_of(1, 48, 1), *weights(128, 48, 1), f)
+    with pytest.raises(RuntimeError, match='maximum'):
+        call(rows_of(1, 32800, 1), *weights(2, 32800, 1), f)
+
+
+def test_refusals_without_a_gpu():
+    import ctypes
+    from thunderworld_b200 import _lib
+    lib = _lib.load()
+    assert lib.tw_matvec(None, None) == 1 and lib.tw_matvec(ctypes.byref(_lib.MatvecArgs()), None) == 1
+    ok = dict(x=256, x_stride=64, codes=256, scales=256, factor=256, out=256, rows=1, n=128, k=128)
+    for bad, status in ((dict(rows=0), 1), (dict(n=0), 1), (dict(k=-32), 1), (dict(rows=33), 9), (dict(k=40), 2), (dict(k=32800), 9),
+                        (dict(x=264), 3), (dict(x_stride=60), 3), (dict(codes=260), 3), (dict(slots=1), 1), (dict(slots=-1), 1),
+                        (dict(slots=1, wr=256, wrs=256), 1), (dict(slots=1, wr=256, wrs=256, dense=1, n=130), 2), (dict(entries=-1), 1)):
+        assert lib.tw_matvec(ctypes.byref(_lib.MatvecArgs(**(ok | bad))), None) == status, bad

@@ -53,6 +53,12 @@ class AttentionArgs(ctypes.Structure):
                                   'pv_terms')]
 
 
+class MatvecArgs(ctypes.Structure):
+    _fields_ = [('x', _vp), ('x_stride', _ll)] + \
+               [(n, _vp) for n in ('prescale', 'codes', 'scales', 'factor', 'bias', 'wr', 'wrs', 'wi', 'off', 'wloc', 'out')] + \
+               [(n, _i) for n in ('rows', 'n', 'k', 'slots', 'entries', 'shared', 'dense', 'out_f32')]
+
+
 _lib = None
 
 
@@ -100,6 +106,7 @@ def load():
     lib.tw_gate_residual_norm.argtypes = [_vp] * 4 + [_i, _f] + [_vp] * 6 + [_i] * 3 + [_f, _vp]
     lib.tw_gate_residual_norm.restype = _i
     lib.tw_capture_id.argtypes = [_vp]; lib.tw_capture_id.restype = ctypes.c_ulonglong
+    lib.tw_matvec.argtypes = [ctypes.POINTER(MatvecArgs), _vp]; lib.tw_matvec.restype = _i
     _lib = lib
     return lib
 
@@ -118,4 +125,4 @@ EXPORTS = ('tw_status', 'tw_abi_version', 'tw_quantize_workspace', 'tw_quantize'
            'tw_quantize_static_max_tiles', 'tw_swizzle_scales', 'tw_activation_rank', 'tw_selftest_bounded_wait',
            'tw_workspace', 'tw_fused', 'tw_fused_tile_n', 'tw_pack_rows', 'tw_select_tiles', 'tw_attention',
            'tw_attention_workspace', 'tw_activate', 'tw_rms_norm', 'tw_rms_norm_heads', 'tw_rope_heads', 'tw_gate_residual',
-           'tw_gate_residual_norm', 'tw_capture_id')
+           'tw_gate_residual_norm', 'tw_capture_id', 'tw_matvec')

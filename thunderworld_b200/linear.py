@@ -118,3 +118,9 @@ class FP4Linear(torch.nn.Module):
         out = ops.fused_gemm(m, n, k, packed, self.weight_codes, self._scales_swz, packed.alpha, na=na, mask=mask,
                              ws=self.weight_scales, mask_per_n=mask is not None, bias=self.bias)
         return out.reshape(*x.shape[:-1], n)
+
+    def matvec(self, x, *, out_dtype=torch.bfloat16):
+        """The layer for a token at a time: at most 32 rows [..., K], which stay BF16 (no activation planes, hence nothing to
+        repair); the same weights, prescale and bias as forward()."""
+        return ops.fp4_matvec(x, self.weight_codes, self.weight_scales, self.weight_global_scale, prescale=self.prescale,
+                              bias=self.bias, out_dtype=out_dtype)

@@ -91,6 +91,13 @@ class Native:
             raise ValueError('expected contiguous BF16 activation on the packed-weight device')
         return self.run_packed(x, self.pack(x))
 
+    def matvec(self, x, bias=None, out=None):
+        """The operator for a token at a time: at most 32 rows [..., K], which stay BF16, against W0 and the selected W1
+        tiles (the terms of a full activation repair with the cross term, without the activation's own rounding)."""
+        bank = dict(wr=self.wr, wrs=self.wrs, wi=self.wi, off=self.off, wloc=self.wloc, shared=self.shared_bank,
+                    dense=self.dense_w) if self.hasw else {}
+        return ops.fp4_matvec(x, self.wc, self.ws, self.wg, prescale=self.d, bias=bias, out=out, **bank)
+
     @property
     def residual_weight_bytes(self):
         return sum(t.numel() * t.element_size() for t in (self.wr, self.wrs, self.wi, self.off)) if self.hasw else 0

@@ -45,6 +45,14 @@ def _stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+_same_device = nullcontext()
+
+
+def _device(device):
+    """Context that makes `device` current; nothing to do, and nothing done, when it is."""
+    return _same_device if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 @dataclass
 class Packed:
     """Quantized activation: the reference's (codes, scales, factor, mp) tuple plus the atom-layout
@@ -197,6 +205,77 @@ def fused_gemm(m, n, k, packed, wc, ws_swz, alpha, *, na=0, mask=None, wr=None, 
     return (out, stats) if want_stats else out
 
 
+MATVEC_ROWS = 32
+
+
+def fp4_matvec(x, codes, scales, factor, *, prescale=None, bias=None, wr=None, wrs=None, wi=None, off=None, wloc=None,
+               shared=False, dense=False, out_dtype=torch.bfloat16, out=None):
+    """Product of a few rows (at most 32) with packed NVFP4 weights, for a token at a time: x bf16 [..., K] stays bf16.
+
+    y = factor * (bf16(x * prescale) @ W.T) + bias, W = codes [N, K/2] x E4M3 scales [N, K/16] plus the W1 tiles of a bank
+    (wr [slots, 128, 64], wrs [slots, 128, 8]; wi, off, wloc, shared, dense as in fused_gemm), sums of 32 bits, one rounding.
+    factor: float32 scalar tensor; prescale float32 [K]; bias bf16 [N]; out_dtype bfloat16 or float32. Any N, K a multiple of
+    32 up to 32768; with a bank both multiples of 128. One launch (two for more than 16 rows of a K above 21 k)."""
+    if x.ndim < 1 or x.dtype is not torch.bfloat16 or not x.is_cuda:
+        raise ValueError('expected CUDA BF16 rows [..., K]')
+    if codes.ndim != 2 or codes.dtype is not torch.uint8 or not codes.is_contiguous():
+        raise ValueError('codes must be contiguous uint8 [N,K/2]')
+    n, k = codes.shape[0], codes.shape[1] * 2
+    dev = x.device
+    if x.shape[-1] != k:
+        raise ValueError(f'expected {k} values per row')
+    if tuple(scales.shape) != (n, k // 16) or scales.dtype is not torch.float8_e4m3fn or not scales.is_contiguous():
+        raise ValueError('scales must be contiguous E4M3 [N,K/16]')
+    if factor.dtype is not torch.float32 or factor.numel() != 1:
+        raise ValueError('factor must be one float32 value')
+    if prescale is not None and (tuple(prescale.shape) != (k,) or prescale.dtype is not torch.float32 or not prescale.is_contiguous()):
+        raise ValueError('prescale must be contiguous float32 [K]')
+    if bias is not None and (tuple(bias.shape) != (n,) or bias.dtype is not torch.bfloat16 or not bias.is_contiguous()):
+        raise ValueError('bias must be contiguous BF16 [N]')
+    if out_dtype is not torch.bfloat16 and out_dtype is not torch.float32:
+        raise ValueError('out_dtype must be bfloat16 or float32')
+    rows = x.numel() // k if k else 0
+    if not rows or not n:
+        raise ValueError('empty activation rows or weights are unsupported')
+    if rows > MATVEC_ROWS:
+        raise ValueError(f'at most {MATVEC_ROWS} rows; more go through the quantizer and fused_gemm')
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise RuntimeError('fp4_matvec is inference-only; use torch.inference_mode()')
+    slots = 0 if wr is None else wr.shape[0]
+    if slots:
+        if n % 128 or k % 128:
+            raise ValueError('a W1 bank needs N and K to be multiples of 128')
+        if tuple(wr.shape) != (slots, 128, 64) or wr.dtype is not torch.uint8 or not wr.is_contiguous():
+            raise ValueError('wr must be contiguous uint8 [slots,128,64]')
+        if wrs is None or wrs.numel() != slots * 1024 or wrs.element_size() != 1 or not wrs.is_contiguous():
+            raise ValueError('wrs must be contiguous E4M3 [slots,128,8]')
+        if not dense:
+            for t, name in ((wi, 'wi'), (off, 'off')) + (((wloc, 'wloc'),) if shared else ()):
+                if t is None or t.dtype is not torch.int32 or not t.is_contiguous():
+                    raise ValueError(f'{name} must be contiguous int32')
+            if off.numel() != n // 128 + 1 or (shared and wloc.numel() != wi.numel()):
+                raise ValueError('off must hold N/128 + 1 offsets and wloc one position per entry of wi')
+    for t in (codes, scales, factor, prescale, bias, wr, wrs, wi, off, wloc):
+        if t is not None and t.device != dev:
+            raise ValueError('activation and packed weights must share a CUDA device')
+    require_sm100(dev)
+    flat = x if x.ndim == 2 else x.reshape(-1, k)
+    if flat.stride(1) != 1 or (rows > 1 and flat.stride(0) % 8) or flat.data_ptr() % 16:
+        flat = flat.clone(memory_format=torch.contiguous_format)
+    shape = (*x.shape[:-1], n)
+    if out is None:
+        out = torch.empty(shape, device=dev, dtype=out_dtype)
+    elif tuple(out.shape) != shape or out.dtype is not out_dtype or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f'out must be contiguous {out_dtype} {shape} on the device of x')
+    args = _lib.MatvecArgs(flat.data_ptr(), flat.stride(0) if rows > 1 else k, _ptr(prescale), codes.data_ptr(), scales.data_ptr(),
+                           factor.data_ptr(), _ptr(bias), _ptr(wr) if slots else None, _ptr(wrs) if slots else None, _ptr(wi),
+                           _ptr(off), _ptr(wloc), out.data_ptr(), rows, n, k, slots, 0 if wi is None else wi.numel(),
+                           int(shared), int(dense), int(out_dtype is torch.float32))
+    with _device(dev):
+        _lib.check(_lib.load().tw_matvec(ctypes.byref(args), _stream(dev)))
+    return out
+
+
 STATUS_KEYS = {'g': 0, 'a': 0, 'q': 8}   # workspace -> byte offset of its device status word: fused GEMM, attention, quantizer
 
 
@@ -339,14 +418,6 @@ def _scratch(device, stream):
     if held is None or held[0] != capture:
         held = _stream_scratch[key] = (capture, torch.zeros(8, device=device, dtype=torch.uint8))
     return held[1]
-
-
-_same_device = nullcontext()
-
-
-def _device(device):
-    """Context that makes `device` current; nothing to do, and nothing done, when it is."""
-    return _same_device if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def _overlap(a, b):
