@@ -140,7 +140,7 @@ typedef struct TwMatvecArgs {
   const void* x;            /* bf16, row r at x + r * x_stride, 16-byte aligned rows */
   long long x_stride;       /* elements, a multiple of 8 */
   const float* prescale;    /* [k] or NULL */
-  const uint8_t *codes, *scales;   /* [n, k/2], [n, k/16] row-major E4M3 */
+  const uint8_t *codes, *scales;   /* [n, k/2], [n, k/16] row-major E4M3; 16-byte and 8-byte aligned, as wr and wrs */
   const float* factor;      /* device scalar */
   const void* bias;         /* bf16 [n] or NULL */
   const uint8_t *wr, *wrs;  /* bank codes [slots, 128, 64] / scales [slots, 128, 8], or NULL */

@@ -11,18 +11,29 @@
 // scales of each; four lanes cover a K128 block of a row, and each lane's 32 k-values may sit in any k-slot of the
 // instruction, because x is laid out alike. A byte of codes is one conversion to two f16 (cvt.rn.f16x2.e2m1x2,
 // one per cycle and scheduler measured; masks and shifts take 2.4 times as long) and one packed multiplication by the scale.
-// The eight warps of a CTA take the K128 blocks of a 16-row tile in turn, four blocks of each warp in flight, and add
-// up in shared memory; a CTA owns consecutive tiles and loads across their borders. Where there are fewer tiles than CTAs fit, or x is too
-// large for a CTA's shared memory, the CTAs of a cluster split K and add up through distributed shared memory: no workspace, and
-// sums of a fixed order.
+// A warp owns 16 rows and runs over its CTA's part of K in quads of four blocks, which it copies to a ring of its own in shared
+// memory, two quads of 4.6 KB, across the borders of its tiles: two CTAs of eight warps have up to 148 KB per SM on the way. A lane
+// copies what it reads itself, so that the copies have immediate offsets: the instructions beside the decoding count (the
+// conversions and all integer work share a half-rate pipe). Rows and x columns that do not exist repeat the last one; their
+// sums are never read. The CTAs of a cluster hold the parts of K: each stages (and scales) only its part of x, and sends
+// its sums of 128 rows to their owners through distributed shared memory, one cluster barrier per 128 rows, waited for after the
+// next 128 rows' products. No workspace, no atomics on sums: the order is fixed.
+//
+// Measured (B200, weights from HBM, graph replay): 1 x 24576 x 6144 24.0 us (3.5 TB/s), 1 x 12288 x 4096 13.4 us, 8 x 16384 x 4096
+// 17.8 us, 1 x 2048 x 2048 5.2 us. Without the products the 24576 x 6144 case streams at 6.3 TB/s, without the copies it takes as
+// long as with both: the decoding's instructions (106 per block of 2048 weights, at half an issue per cycle and scheduler) are
+// what bounds the large cases, start (launch, x to f16: 4 us) and join the small ones.
+#include <atomic>
 #include "tw_common.cuh"
 #include "../../include/twb200.h"
 
 namespace {
 
-constexpr int WARPS = 8, THREADS = WARPS * 32, DEPTH = 4;
-constexpr int COL_PITCH = 20;       // floats per x row of a warp's 16-row partial tile: bank = 8 t + g, no conflicts
-constexpr int MAX_TILES = 64;       // 16-row tiles per CTA; bounds the shared-memory lists of bank tiles
+constexpr int WARPS = 8, THREADS = WARPS * 32;
+constexpr int SCALE_PITCH = 40;     // bytes per row of a quad's scales: 32, in up to five aligned words; a load's banks are all different
+constexpr int QUAD = 16 * 256 + 16 * SCALE_PITCH;    // bytes of a ring slot: codes by lane, then scales
+constexpr int MAX_ROUNDS = 32;      // N128 blocks per cluster; bounds the shared-memory lists of bank tiles
+constexpr int MOST_SMEM = 224 * 1024, PAIR_SMEM = 112 * 1024;      // of one CTA on an SM, of each of two
 
 struct Params {
   const __nv_bfloat16* x; long long x_stride;
@@ -33,13 +44,15 @@ struct Params {
   const uint8_t *wr, *wrs;
   const int *off, *wi, *wloc;
   void* out;
-  int rows, n, k, kb, tiles, groups, ksplit, slots, entries, shared, dense, out_f32, list_blocks;
+  int rows, n, k, kb, nb, groups, ksplit, slots, entries, shared, dense, out_f32;
 };
 
-__device__ __forceinline__ uint4 load_codes(const uint8_t* p) {          // read once: keep it out of L1
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+// The first `bytes` (0 ... 8) from global memory, zeros behind them.
+__device__ __forceinline__ void copy8(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 // Eight codes -> four f16 pairs, low nibble first.
 __device__ __forceinline__ void decode8(uint32_t w, __half2 scale, uint32_t (&o)[4]) {
@@ -65,44 +78,53 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float peer_load(const float* own, uint32_t rank) {
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void peer_store(float* own, uint32_t rank, float v) {      // at the same place of another CTA of the cluster
   uint32_t addr;
-  float v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(tw::smem_u32(own)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
-// Where a warp is in its sequence of K128 blocks: all W0 blocks of a tile, then the tile's bank blocks, then the next tile.
-struct Cursor {
-  int tile, at;
-};
+// Floats of a buffer for a round's sums: as many shares of them as there are ranks, rounded up; even.
+__device__ __host__ __forceinline__ int sum_floats(int rows, int ksplit) { return (rows * 128 + ksplit * ksplit + 1) & ~1; }
+// Bytes of a row of x in shared memory: a block's 64 chunks of 16 bytes by word of codes and lane, and 64 bytes that put the
+// eight rows that a warp reads at once into different banks.
+__device__ __host__ __forceinline__ int x_pitch(int blocks) { return blocks * 256 + 64; }
+// Where chunk c (8 values: word c & 3 of lane (c & 15) / 4 of block c / 16) of a row lies.
+__device__ __forceinline__ int x_chunk(int c) { return (c >> 4) * 256 + (c & 3) * 64 + ((c & 15) >> 2) * 16; }
 
 template <int MT, bool BANK>     // MT: groups of 8 x rows
-__global__ void __launch_bounds__(THREADS, 2) matvec_kernel(Params p) {
+__global__ void __launch_bounds__(THREADS, 2) matvec_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(16) uint8_t dynamic[];
   __shared__ unsigned peak[32];
   __shared__ float unscale[32];
+  __shared__ int counts[MAX_ROUNDS];               // bank blocks of a round
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rank = p.ksplit > 1 ? (int)cluster_rank() : 0, group = blockIdx.x / p.ksplit;
-  const int kb0 = (int)((long long)p.kb * rank / p.ksplit), nkb = (int)((long long)p.kb * (rank + 1) / p.ksplit) - kb0;
-  const int max_kb = (p.kb + p.ksplit - 1) / p.ksplit;
-  const int tile0 = (int)((long long)p.tiles * group / p.groups), tile1 = (int)((long long)p.tiles * (group + 1) / p.groups);
-  uint4* xs = reinterpret_cast<uint4*>(dynamic);                                  // [max_kb][4 words][rows][4 lanes]
-  float* red = reinterpret_cast<float*>(xs + (size_t)max_kb * 16 * p.rows);       // [2][WARPS][8 MT][COL_PITCH]
-  float* part = red + 2 * WARPS * 8 * MT * COL_PITCH;                             // [2][8 MT][16], only with ksplit > 1
-  int2* list = reinterpret_cast<int2*>(part + (p.ksplit > 1 ? 2 * 8 * MT * 16 : 0));   // [list_blocks][max_kb], only with a bank
-  int* counts = reinterpret_cast<int*>(list + (BANK ? (size_t)p.list_blocks * max_kb : 0));
-  const int nb0 = tile0 >> 3;
+  const int kb0 = p.kb * rank / p.ksplit, nkb = p.kb * (rank + 1) / p.ksplit - kb0, max_kb = (p.kb + p.ksplit - 1) / p.ksplit;
+  const int nb0 = (int)((long long)p.nb * group / p.groups), rounds = (int)((long long)p.nb * (group + 1) / p.groups) - nb0;
+  const int pitch = x_pitch(max_kb);
+  uint8_t* ring = dynamic + warp * 2 * QUAD;                                                     // [WARPS][2][QUAD]
+  uint8_t* xs = dynamic + WARPS * 2 * QUAD;                                                      // [rows][pitch]
+  float* landing = reinterpret_cast<float*>(xs + p.rows * pitch);                                // [2][ranks][rows * 128 / ranks]
+  int2* list = reinterpret_cast<int2*>(landing + 2 * sum_floats(p.rows, p.ksplit));              // [rounds][max_kb], only with a bank
 
+  if (p.ksplit > 1) cluster_arrive();              // waited for before the first store to a peer: it has to be running
+  // this CTA's part of x on its way to shared memory while the weights' first blocks are fetched
+  const int chunks = nkb * 16, items = p.rows * chunks;                           // of 8 values; 16 lanes have chunks of one row
+  for (int i = threadIdx.x; i < items; i += THREADS) {
+    const int r = i / chunks, c = i - r * chunks, kk = kb0 * 128 + c * 8;
+    uint8_t* to = xs + r * pitch + x_chunk(c);
+    if (kk < p.k) copy16(tw::smem_u32(to), p.x + r * p.x_stride + kk);
+    else *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);                  // k % 32 == 0; zeros behind it
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  if (threadIdx.x < 32) peak[threadIdx.x] = 0;
   if (BANK) {
-    // the bank tiles of this CTA's N128 blocks that lie in its part of K: {x block, bank position}
-    const int last = tile1 > tile0 ? (tile1 - 1) >> 3 : nb0 - 1;
-    for (int nb = nb0 + warp; nb <= last; nb += WARPS) {
-      int2* mine = list + (size_t)(nb - nb0) * max_kb;
+    // the bank tiles of this cluster's N128 blocks that lie in this CTA's part of K: {block, bank position}
+    for (int j = warp; j < rounds; j += WARPS) {
+      const int nb = nb0 + j;
       int filled = 0;
       const int begin = p.dense ? nb * p.kb : max(__ldg(p.off + nb), 0);
       const int end = p.dense ? begin + p.kb : min(__ldg(p.off + nb + 1), p.entries);
@@ -116,201 +138,328 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_kernel(Params p) {
         const bool take = block >= 0 && block < nkb && loc >= 0 && loc < p.slots;
         const unsigned who = __ballot_sync(0xffffffffu, take);
         const int slot = filled + __popc(who & ((1u << lane) - 1u));
-        if (take && slot < max_kb) mine[slot] = make_int2(block, loc);
+        if (take && slot < max_kb) list[(size_t)j * max_kb + slot] = make_int2(block, loc);
         filled += __popc(who);
       }
-      if (lane == 0) counts[nb - nb0] = filled < max_kb ? filled : max_kb;
+      if (lane == 0) counts[j] = filled < max_kb ? filled : max_kb;
     }
-    __syncthreads();
   }
+  __syncthreads();
 
-  // ---- the stream of weight blocks: registers hold DEPTH of them --------------------------------------------------
-  uint4 code[DEPTH][2];
-  uint32_t scale[DEPTH][2];
-  int block_of[DEPTH];                 // x block, or -1 for nothing to add
-  bool ends[DEPTH];                    // the warp's last block of the tile
-  const int own = nkb > warp ? (nkb - warp + WARPS - 1) / WARPS : 0;              // this warp's W0 blocks of a tile
-  Cursor cur{tile0, 0};
-  auto fetch = [&](int slot) {
-    code[slot][0] = code[slot][1] = make_uint4(0, 0, 0, 0);
-    scale[slot][0] = scale[slot][1] = 0;
-    block_of[slot] = -1;
-    ends[slot] = true;
-    if (cur.tile >= tile1) return;
-    int steps = own;
-    if (BANK) {
-      const int count = counts[(cur.tile >> 3) - nb0];
-      steps += count > warp ? (count - warp + WARPS - 1) / WARPS : 0;
-    }
-    if (cur.at < steps) {
-      const int row0 = cur.tile * 16 + g;
-      if (!BANK || cur.at < own) {
-        const int block = warp + cur.at * WARPS, kk = (kb0 + block) * 128 + t * 32;
-        block_of[slot] = block;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = row0 + 8 * h;
-          if (row < p.n && kk < p.k) {
-            code[slot][h] = load_codes(p.codes + (size_t)row * (p.k / 2) + kk / 2);
-            scale[slot][h] = __ldg(reinterpret_cast<const uint16_t*>(p.scales + (size_t)row * (p.k / 16) + kk / 16));
-          }
-        }
-      } else {
-        const int2 e = list[(size_t)((cur.tile >> 3) - nb0) * max_kb + warp + (cur.at - own) * WARPS];
-        block_of[slot] = e.x;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {                 // n and k are multiples of 128 with a bank
-          const size_t row = (size_t)e.y * 128 + ((row0 + 8 * h) & 127);
-          code[slot][h] = load_codes(p.wr + row * 64 + t * 16);
-          scale[slot][h] = __ldg(reinterpret_cast<const uint16_t*>(p.wrs + row * 8 + t * 2));
-        }
-      }
-    }
-    if (++cur.at >= steps) { ++cur.tile; cur.at = 0; } else ends[slot] = false;
+  // ---- the stream of weight blocks: W0's of this part of K, then the bank's, then the next round ----------------------
+  // Two cursors run over it quad by quad: one fetches, one, two quads behind, multiplies.
+  const size_t code_pitch = p.k / 2, scale_pitch = p.k / 16;
+  struct Cursor { int round, at, w0, bank; };      // blocks fetched or multiplied of the round's w0 + bank
+  auto open = [&](Cursor& c) {
+    c.w0 = c.round < rounds && (nb0 + c.round) * 128 + warp * 16 < p.n ? nkb : 0;
+    c.bank = BANK && c.w0 ? counts[c.round] : 0;
+    c.at = 0;
   };
+  // blocks of the quad that the cursor is at: four, or what is left of W0's or of the bank's
+  auto width = [&](const Cursor& c) { return min((!BANK || c.at < c.w0 ? c.w0 : c.w0 + c.bank) - c.at, 4); };
+  Cursor in{0, 0, 0, 0};
+  // a lane copies the 16 bytes of each block and row that it will read; the scales as the aligned words that hold a row's: words
+  // 2 (lane & 1) and one more of row lane / 2, and, where rows do not begin on one, the fifth word of row lane
+  const uint32_t ring_at = tw::smem_u32(ring), code_to = ring_at + lane * 16;
+  const uint32_t scale_to = ring_at + 4096 + (lane >> 1) * SCALE_PITCH + (lane & 1) * 16, fifth_to = ring_at + 4096 + lane * SCALE_PITCH + 32;
+  const bool fifth = scale_pitch % 8 && lane < 16;
+  // lanes whose 32 k of the last block lie behind K repeat the block's first 32 (x is zero there)
+  const int last_block = p.kb - 1 - kb0, tail = last_block < nkb && (kb0 + last_block) * 128 + t * 32 >= p.k ? t * 16 : 0;
+  const uint8_t *c0, *c8, *s0, *s32;               // where the round's next quad begins for this lane
+  auto aligned = [](const uint8_t* at) { return reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(at) & ~(uintptr_t)7); };
+  auto point = [&]() {
+    const int row0 = (nb0 + in.round) * 128 + warp * 16;
+    c0 = p.codes + min(row0 + g, p.n - 1) * code_pitch + kb0 * 64 + t * 16;
+    c8 = p.codes + min(row0 + g + 8, p.n - 1) * code_pitch + kb0 * 64 + t * 16;
+    s0 = aligned(p.scales + min(row0 + (lane >> 1), p.n - 1) * scale_pitch + kb0 * 8) + (lane & 1) * 16;
+    s32 = aligned(p.scales + min(row0 + (lane & 15), p.n - 1) * scale_pitch + kb0 * 8) + 32;
+  };
+  auto fetch = [&](int slot) {
+    const int n = width(in);
+    const uint32_t offset = slot * QUAD;
+    if (n > 0 && (!BANK || in.at < in.w0)) {
+      if (n == 4 && in.at + 3 < last_block) {                        // the usual quad
 #pragma unroll
-  for (int s = 0; s < DEPTH; ++s) fetch(s);
-
-  // ---- x: bf16(x d) to shared memory in the order the lanes read it, then to scaled f16 in place --------------------
-  if (threadIdx.x < 32) peak[threadIdx.x] = 0;
-  __syncthreads();
-  const int chunks = nkb * 16;                                                    // of 8 values
-  for (int r = 0; r < p.rows; ++r) {
-    unsigned top = 0;
-    for (int c = threadIdx.x; c < chunks; c += THREADS) {
-      const int kk = kb0 * 128 + c * 8;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (kk < p.k) {                                                             // k % 32 == 0
-        v = __ldg(reinterpret_cast<const uint4*>(p.x + r * p.x_stride + kk));
-        uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (p.prescale) {
-            const float2 d = __ldg(reinterpret_cast<const float2*>(p.prescale + kk + 2 * i));
-            const __nv_bfloat162 b = __floats2bfloat162_rn(__fmul_rn(tw::bf16_bits_to_float(w[i] & 0xffffu), d.x),
-                                                           __fmul_rn(tw::bf16_bits_to_float(w[i] >> 16), d.y));
-            w[i] = *reinterpret_cast<const uint32_t*>(&b);
-          }
-          const unsigned lo = (w[i] & 0x7fffu) << 16, hi = w[i] & 0x7fff0000u;
-          if (lo < 0x7f800000u) top = max(top, lo);                               // finite values only
-          if (hi < 0x7f800000u) top = max(top, hi);
+        for (int j = 0; j < 4; ++j) {
+          copy16(code_to + offset + j * 1024, c0 + j * 64);
+          copy16(code_to + offset + j * 1024 + 512, c8 + j * 64);
         }
-        v = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-      // chunk c of a block: lane t = (c & 15) / 4 holds k 32 t ... 32 t + 31, word i = c & 3 of its 16 bytes of codes
-      xs[(size_t)(((c >> 4) * 4 + (c & 3)) * p.rows + r) * 4 + ((c & 15) >> 2)] = v;
-    }
+        copy8(scale_to + offset, s0, 8);
+        copy8(scale_to + offset + 8, s0 + 8, 8);
+        if (fifth) copy8(fifth_to + offset, s32, 8);
+      } else {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0 && top) atomicMax(&peak[r], top);
+        for (int j = 0; j < 4; ++j) {
+          if (j < n) {
+            const int back = in.at + j == last_block ? tail : 0;
+            copy16(code_to + offset + j * 1024, c0 + j * 64 - back);
+            copy16(code_to + offset + j * 1024 + 512, c8 + j * 64 - back);
+          }
+        }
+        // what lies behind the row's end is zero
+        const int row0 = (nb0 + in.round) * 128 + warp * 16;
+        auto word = [&](uint32_t to, const uint8_t* from, int r) {
+          const long long rest = p.scales + (min(row0 + r, p.n - 1) + 1) * scale_pitch - from;
+          const int size = (int)(rest < 0 ? 0 : rest > 8 ? 8 : rest);
+          copy8(to + offset, size ? from : p.scales, size);
+        };
+        word(scale_to, s0, lane >> 1);
+        word(scale_to + 8, s0 + 8, lane >> 1);
+        if (fifth) word(fifth_to, s32, lane);
+      }
+      c0 += 256; c8 += 256; s0 += 32; s32 += 32;
+    } else if (BANK && n > 0) {                    // n and k are multiples of 128; a bank tile's rows lie one behind the other
+      const int2* entry = list + (size_t)in.round * max_kb + in.at - in.w0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (j < n) {
+          const size_t row = (size_t)entry[j].y * 128 + warp * 16;
+          copy16(code_to + offset + j * 1024, p.wr + (row + g) * 64 + t * 16);
+          copy16(code_to + offset + j * 1024 + 512, p.wr + (row + g + 8) * 64 + t * 16);
+          if (lane < 16) copy8(ring_at + offset + 4096 + lane * SCALE_PITCH + j * 8, p.wrs + (row + lane) * 8, 8);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    in.at += n;
+    if (in.at >= in.w0 + in.bank) {    // a round without a block for this warp takes one empty quad all the same
+      ++in.round;
+      open(in);
+      if (in.w0 > 0) point();
+    }
+  };
+  open(in);
+  if (in.w0 > 0) point();
+  fetch(0);
+
+  // ---- x d, rounded to bf16, in the order the lanes read it; then scaled f16 in place ------------------------------
+  asm volatile("cp.async.wait_group 1;" ::: "memory");         // a thread's own chunks: nobody else reads them before the barrier
+  for (int i = threadIdx.x; i < items; i += THREADS) {
+    const int r = i / chunks, c = i - r * chunks, kk = kb0 * 128 + c * 8;
+    uint4* to = reinterpret_cast<uint4*>(xs + r * pitch + x_chunk(c));
+    const uint4 v = *to;
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    if (p.prescale && kk < p.k) {
+      const float4 d0 = __ldg(reinterpret_cast<const float4*>(p.prescale + kk)), d1 = __ldg(reinterpret_cast<const float4*>(p.prescale + kk) + 1);
+      const float d[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(__fmul_rn(tw::bf16_bits_to_float(w[j] & 0xffffu), d[2 * j]),
+                                                       __fmul_rn(tw::bf16_bits_to_float(w[j] >> 16), d[2 * j + 1]));
+        w[j] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+      *to = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    unsigned top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const unsigned lo = (w[j] & 0x7fffu) << 16, hi = w[j] & 0x7fff0000u;
+      top = max(top, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));        // finite values only
+    }
+    // 16 lanes hold chunks of one row, and enter together: items is a multiple of 16
+    const unsigned mates = 0xffffu << (lane & 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mates, top, o));
+    if ((lane & 15) == 0 && top) atomicMax(&peak[r], top);
   }
+  fetch(1);
   __syncthreads();
-  for (int r = 0; r < p.rows; ++r) {
+  for (int i = threadIdx.x; i < items; i += THREADS) {
+    const int r = i / chunks, c = i - r * chunks;
     // 2^shift brings the largest value to [2^14, 2^15); an all-zero row stays, and 2^shift stays a normal number
     const int shift = peak[r] ? min(14 - ((int)(peak[r] >> 23) - 127), 126) : 0;
     const float up = __uint_as_float((unsigned)(127 + shift) << 23);
-    if (threadIdx.x == 0) unscale[r] = __uint_as_float((unsigned)(127 - shift) << 23);
-    for (int c = threadIdx.x; c < chunks; c += THREADS) {
-      uint4* at = xs + (size_t)(((c >> 4) * 4 + (c & 3)) * p.rows + r) * 4 + ((c & 15) >> 2);
-      const uint4 v = *at;
-      uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    if (c == 0) unscale[r] = __uint_as_float((unsigned)(127 - shift) << 23);
+    uint4* to = reinterpret_cast<uint4*>(xs + r * pitch + x_chunk(c));
+    const uint4 v = *to;
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const __half2 h = __floats2half2_rn(tw::bf16_bits_to_float(w[i] & 0xffffu) * up, tw::bf16_bits_to_float(w[i] >> 16) * up);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-      }
-      *at = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int j = 0; j < 4; ++j) {
+      const __half2 h = __floats2half2_rn(tw::bf16_bits_to_float(w[j] & 0xffffu) * up, tw::bf16_bits_to_float(w[j] >> 16) * up);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
     }
+    *to = make_uint4(w[0], w[1], w[2], w[3]);
   }
   __syncthreads();
 
   // ---- products --------------------------------------------------------------------------------------------------
   const float factor = __ldg(p.factor);
-  float acc[MT][4];
+  constexpr int CHAINS = MT == 1 ? 2 : 1;          // of dependent additions: one per x group, two where there is one group
+  float acc[MT][CHAINS][4];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
-  int tile = tile0, buffer = 0;
-  while (tile < tile1) {
+  for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int s = 0; s < DEPTH; ++s) {
-      if (tile < tile1) {
-        if (block_of[s] >= 0) {
-          __half2 sc[2][2];
-          decode_scales(scale[s][0], sc[0][0], sc[0][1]);
-          decode_scales(scale[s][1], sc[1][0], sc[1][1]);
-          const uint32_t w[2][4] = {{code[s][0].x, code[s][0].y, code[s][0].z, code[s][0].w},
-                                    {code[s][1].x, code[s][1].y, code[s][1].z, code[s][1].w}};
-          const uint4* xb = xs + (size_t)block_of[s] * 16 * p.rows + lane;
+    for (int h = 0; h < CHAINS; ++h) acc[m][h][0] = acc[m][h][1] = acc[m][h][2] = acc[m][h][3] = 0.f;
+  const uint8_t* x_lane[MT];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t a[2][4];
-            decode8(w[0][i], sc[0][i >> 1], a[0]);
-            decode8(w[1][i], sc[1][i >> 1], a[1]);
+  for (int m = 0; m < MT; ++m) x_lane[m] = xs + min(m * 8 + g, p.rows - 1) * pitch + t * 16;
+  auto multiply = [&](const uint8_t* codes, const uint8_t* low, const uint8_t* high, int block) {
+    const uint4 first = *reinterpret_cast<const uint4*>(codes), second = *reinterpret_cast<const uint4*>(codes + 512);
+    __half2 sc[2][2];
+    decode_scales(*reinterpret_cast<const uint16_t*>(low), sc[0][0], sc[0][1]);
+    decode_scales(*reinterpret_cast<const uint16_t*>(high), sc[1][0], sc[1][1]);
+    const uint32_t w[2][4] = {{first.x, first.y, first.z, first.w}, {second.x, second.y, second.z, second.w}};
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              const uint4 b = m * 8 + g < p.rows ? xb[i * 4 * p.rows + m * 32] : make_uint4(0, 0, 0, 0);
-              mma_f16(acc[m], a[0][0], a[1][0], a[0][1], a[1][1], b.x, b.y);
-              mma_f16(acc[m], a[0][2], a[1][2], a[0][3], a[1][3], b.z, b.w);
-            }
-          }
-        }
-        const bool end = ends[s];
-        fetch(s);
-        if (end) {
-          float* mine = red + ((size_t)buffer * WARPS + warp) * 8 * MT * COL_PITCH;
+    for (int i = 0; i < 4; ++i) {
+      uint32_t a[2][4];
+      decode8(w[0][i], sc[0][i >> 1], a[0]);
+      decode8(w[1][i], sc[1][i >> 1], a[1]);
 #pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            float* c = mine + (m * 8 + 2 * t) * COL_PITCH + g;
-            c[0] = acc[m][0]; c[COL_PITCH] = acc[m][1]; c[8] = acc[m][2]; c[COL_PITCH + 8] = acc[m][3];
-            acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
-          }
-          __syncthreads();               // the other buffer is written next: one barrier per tile is enough
-          float sum[(MT * 128 + THREADS - 1) / THREADS];
-#pragma unroll
-          for (int o = 0; o < (MT * 128 + THREADS - 1) / THREADS; ++o) {
-            const int e = threadIdx.x + o * THREADS, col = e >> 4, row = e & 15;
-            sum[o] = 0.f;
-            if (col < p.rows) {
-              const float* from = red + (size_t)buffer * WARPS * 8 * MT * COL_PITCH + col * COL_PITCH + row;
-#pragma unroll
-              for (int w8 = 0; w8 < WARPS; ++w8) sum[o] += from[w8 * 8 * MT * COL_PITCH];
-              sum[o] *= unscale[col];
-              if (p.ksplit > 1) part[buffer * 8 * MT * 16 + e] = sum[o];
-            }
-          }
-          if (p.ksplit > 1) cluster_sync();
-#pragma unroll
-          for (int o = 0; o < (MT * 128 + THREADS - 1) / THREADS; ++o) {
-            const int e = threadIdx.x + o * THREADS, col = e >> 4, row = tile * 16 + (e & 15);
-            if (col < p.rows && row < p.n && (p.ksplit == 1 || col % p.ksplit == rank)) {
-              float y = sum[o];
-              if (p.ksplit > 1) {        // the ranks' sums in their order, whoever adds them
-                y = 0.f;
-                for (int q = 0; q < p.ksplit; ++q) y += peer_load(part + buffer * 8 * MT * 16 + e, q);
-              }
-              y *= factor;
-              if (p.bias) y += __bfloat162float(p.bias[row]);
-              const size_t at = (size_t)col * p.n + row;
-              if (p.out_f32) static_cast<float*>(p.out)[at] = y;
-              else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
-            }
-          }
-          buffer ^= 1;
-          ++tile;
-        }
+      for (int m = 0; m < MT; ++m) {
+        const uint4 b = *reinterpret_cast<const uint4*>(x_lane[m] + block * 256 + i * 64);
+        mma_f16(acc[m][0], a[0][0], a[1][0], a[0][1], a[1][1], b.x, b.y);
+        mma_f16(acc[m][CHAINS - 1], a[0][2], a[1][2], a[0][3], a[1][3], b.z, b.w);
       }
     }
+  };
+  // A round's sums over this CTA's part of K are in `landing`, its owners' share of them from every rank; rank q adds its share,
+  // elements (x row, weight row) q * share ..., in the order of the ranks.
+  const int elements = p.rows * 128, share = (elements + p.ksplit - 1) / p.ksplit, floats = sum_floats(p.rows, p.ksplit);
+  auto join = [&](int done) {
+    const float* from = landing + (done & 1) * floats;
+    for (int j = threadIdx.x; j < share && rank * share + j < elements; j += THREADS) {
+      const int e = rank * share + j, col = e >> 7, row = (nb0 + done) * 128 + (e & 127);
+      if (row >= p.n) continue;
+      float y = 0.f;
+      for (int q = 0; q < p.ksplit; ++q) y += from[q * share + j];
+      y *= factor;
+      if (p.bias) y += __bfloat162float(p.bias[row]);
+      const size_t to = (size_t)col * p.n + row;
+      if (p.out_f32) static_cast<float*>(p.out)[to] = y;
+      else static_cast<__nv_bfloat16*>(p.out)[to] = __float2bfloat16_rn(y);
+    }
+  };
+  Cursor at{0, 0, 0, 0};
+  open(at);
+  int slot = 0;
+  while (at.round < rounds) {
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
+    const uint8_t* codes = ring + slot * QUAD + lane * 16;
+    const int n = width(at);
+    const uint8_t *low = ring + slot * QUAD + 4096 + t * 2 + g * SCALE_PITCH, *high = low + 8 * SCALE_PITCH;
+    if (!BANK || at.at < at.w0) {
+      if (scale_pitch % 8) {             // where a row's scales begin within their first aligned word
+        const int row = (nb0 + at.round) * 128 + warp * 16 + g;
+        low += (min(row, p.n - 1) * (uint32_t)scale_pitch) & 7;
+        high += (min(row + 8, p.n - 1) * (uint32_t)scale_pitch) & 7;
+      }
+      if (n == 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) multiply(codes + j * 1024, low + j * 8, high + j * 8, at.at + j);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+          if (j < n) multiply(codes + j * 1024, low + j * 8, high + j * 8, at.at + j);
+      }
+    } else {
+      const int2* entry = list + (size_t)at.round * max_kb + at.at - at.w0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < n) multiply(codes + j * 1024, low + j * 8, high + j * 8, entry[j].x);
+    }
+    __syncwarp();
+    fetch(slot);
+    slot ^= 1;
+    at.at += n;
+    if (at.at >= at.w0 + at.bank) {
+      if (p.ksplit > 1) {                // the barrier of the round before; at first, the one that says that all ranks run
+        cluster_wait();
+        if (at.round > 0) join(at.round - 1);
+      } else if (at.round > 0) {
+        __syncthreads();
+        join(at.round - 1);
+      }
+      float* mine = landing + (at.round & 1) * floats;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const int col = m * 8 + 2 * t + (h & 1), e = col * 128 + warp * 16 + g + (h >> 1) * 8;
+          const float y = CHAINS == 1 ? acc[m][0][h] : acc[m][0][h] + acc[m][CHAINS - 1][h];
+          if (col < p.rows) {
+            if (p.ksplit > 1) { const int owner = e / share; peer_store(mine + rank * share + e - owner * share, owner, y * unscale[col]); }
+            else mine[e] = y * unscale[col];
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < CHAINS; ++h) acc[m][h][0] = acc[m][h][1] = acc[m][h][2] = acc[m][h][3] = 0.f;
+      }
+      // the other buffer's readers are through before anyone passes the barrier that follows
+      __syncwarp();
+      if (p.ksplit > 1) cluster_arrive();
+      ++at.round;
+      open(at);
+    }
   }
-  if (p.ksplit > 1) cluster_sync();      // nobody leaves while its sums may still be read
+  if (p.ksplit > 1) cluster_wait(); else __syncthreads();
+  if (rounds > 0) join(rounds - 1);
+}
+
+// Clusters of `ksplit` CTAs, one or two CTAs per SM, that run beside each other: asked once per kind, the query takes longer
+// than a launch.
+int fitting_clusters(int ksplit, int per_sm) {
+  static std::atomic<int> known[9][3];
+  int n = known[ksplit][per_sm].load(std::memory_order_relaxed);
+  if (n) return n;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(148 * 2 * ksplit);
+  config.blockDim = dim3(THREADS);
+  config.dynamicSmemBytes = per_sm == 2 ? PAIR_SMEM : MOST_SMEM;
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = ksplit;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  config.attrs = &cluster;
+  config.numAttrs = 1;
+  if (cudaFuncSetAttribute(matvec_kernel<1, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_SMEM) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, matvec_kernel<1, false>, &config) != cudaSuccess || n < 1) {
+    (void)cudaGetLastError();
+    n = 148 * per_sm * 7 / 8 / ksplit;
+  }
+  known[ksplit][per_sm].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+size_t smem_bytes(int rows, int kb, int ksplit, int rounds) {        // rounds: with a bank, else 0
+  const int kbs = (kb + ksplit - 1) / ksplit;
+  return (size_t)WARPS * 2 * QUAD + (size_t)rows * x_pitch(kbs) + (size_t)2 * sum_floats(rows, ksplit) * 4 + (size_t)rounds * kbs * 8;
 }
 
 template <int MT, bool BANK>
-int launch(const Params& p, size_t smem, cudaStream_t stream) {
+int launch(Params p, cudaStream_t stream) {
   auto kernel = matvec_kernel<MT, BANK>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return TW_ERR_LAUNCH;
+  static std::atomic<bool> configured[64];            // the shared-memory opt-in is a per-device attribute of the function
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) { (void)cudaGetLastError(); return TW_ERR_LAUNCH; }
+  if (device >= 64 || !configured[device].load(std::memory_order_relaxed)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_SMEM) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return TW_ERR_LAUNCH;
+    }
+    if (device < 64) configured[device].store(true, std::memory_order_relaxed);
   }
+  // The cluster size that leaves a warp the fewest blocks: rounds of 128 rows times blocks per round, a round's barrier and
+  // sums counted as 2 MT blocks. More clusters than run beside each other would wait for the others; one CTA on an SM
+  // instead of two has half the warps to hide its latencies.
+  int best = 0, best_cost = 1 << 30;
+  size_t smem = 0;
+  for (int ksplit = 1; ksplit <= 8 && ksplit <= p.kb; ++ksplit) {
+    const int kbs = (p.kb + ksplit - 1) / ksplit;
+    for (int per_sm = 2; per_sm >= 1; --per_sm) {
+      int groups = ksplit == 1 ? 148 * per_sm : fitting_clusters(ksplit, per_sm);
+      if (groups > p.nb) groups = p.nb;
+      if (groups < (p.nb + MAX_ROUNDS - 1) / MAX_ROUNDS) groups = (p.nb + MAX_ROUNDS - 1) / MAX_ROUNDS;
+      const int rounds = (p.nb + groups - 1) / groups;
+      const size_t need = smem_bytes(p.rows, p.kb, ksplit, BANK ? rounds : 0);
+      if (need > (size_t)(per_sm == 2 ? PAIR_SMEM : MOST_SMEM)) continue;
+      const int cost = rounds * (kbs + 2 * MT) + p.rows * kbs / 8;
+      if (cost < best_cost) { best = ksplit; best_cost = cost; p.groups = groups; smem = need; }
+      break;
+    }
+  }
+  if (!best) return TW_ERR_TOO_LARGE;
+  p.ksplit = best;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(p.groups * p.ksplit);
   config.blockDim = dim3(THREADS);
@@ -321,7 +470,7 @@ int launch(const Params& p, size_t smem, cudaStream_t stream) {
   cluster.val.clusterDim.x = p.ksplit;
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   config.attrs = &cluster;
-  config.numAttrs = p.ksplit > 1 ? 1 : 0;
+  config.numAttrs = best > 1 ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&config, kernel, p);
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e == cudaSuccess ? TW_OK : TW_ERR_LAUNCH;
@@ -338,8 +487,8 @@ extern "C" int tw_matvec(const TwMatvecArgs* a, void* stream) {
   if (bank && !a->dense && (!a->off || !a->wi || (a->shared && !a->wloc))) return TW_ERR_ARGUMENT;
   if (a->k % 32 || (bank && (a->n % 128 || a->k % 128))) return TW_ERR_SHAPE;
   if (a->rows > 32 || a->k > 32768) return TW_ERR_TOO_LARGE;
-  if (misaligned(a->x, 16) || a->x_stride % 8 || misaligned(a->codes, 16) || misaligned(a->scales, 2) || misaligned(a->factor, 4) ||
-      misaligned(a->prescale, 8) || misaligned(a->bias, 2) || misaligned(a->wr, 16) || misaligned(a->wrs, 2) ||
+  if (misaligned(a->x, 16) || a->x_stride % 8 || misaligned(a->codes, 16) || misaligned(a->scales, 8) || misaligned(a->factor, 4) ||
+      misaligned(a->prescale, 16) || misaligned(a->bias, 2) || misaligned(a->wr, 16) || misaligned(a->wrs, 8) ||
       misaligned(a->out, a->out_f32 ? 4 : 2))
     return TW_ERR_ALIGNMENT;
   Params p = {};
@@ -347,36 +496,20 @@ extern "C" int tw_matvec(const TwMatvecArgs* a, void* stream) {
   p.prescale = a->prescale; p.codes = a->codes; p.scales = a->scales; p.factor = a->factor;
   p.bias = static_cast<const __nv_bfloat16*>(a->bias);
   p.wr = a->wr; p.wrs = a->wrs; p.off = a->off; p.wi = a->wi; p.wloc = a->wloc; p.out = a->out;
-  p.rows = a->rows; p.n = a->n; p.k = a->k; p.kb = (a->k + 127) / 128; p.tiles = (a->n + 15) / 16;
+  p.rows = a->rows; p.n = a->n; p.k = a->k; p.kb = (a->k + 127) / 128; p.nb = (a->n + 127) / 128;
   p.slots = a->slots; p.entries = a->entries; p.shared = a->shared; p.dense = a->dense; p.out_f32 = a->out_f32;
-  // K is split over a cluster until a CTA's part of x leaves room for a second CTA on its SM, and further while the CTAs
-  // still fit beside each other and every warp keeps two K128 blocks of a tile
-  constexpr int ROOM = 104 * 1024, MOST = 220 * 1024;
-  auto bytes = [&](int ksplit, int list_blocks) {
-    const int mt = p.rows <= 8 ? 1 : p.rows <= 16 ? 2 : 4;
-    const size_t kbs = (p.kb + ksplit - 1) / ksplit;
-    return kbs * 256 * p.rows + (size_t)2 * WARPS * 8 * mt * COL_PITCH * 4 + (ksplit > 1 ? (size_t)2 * 8 * mt * 16 * 4 : 0) +
-           (bank ? (size_t)list_blocks * (kbs * 8 + 4) : 0);
-  };
-  if (bytes(8, MAX_TILES / 8 + 2) > MOST) p.rows = 16;       // K > 21 k: more rows go in passes of 16, which always fit
-  const int step = p.rows;
+  // 32 rows at a time, or what fits a cluster: 16 rows for a K above 13 k, 8 for a K above 28 k
+  int most = 32;
+  while (most > 8 && smem_bytes(most, p.kb, p.kb < 8 ? p.kb : 8, bank ? MAX_ROUNDS : 0) > MOST_SMEM) most /= 2;
+  const int passes = (a->rows + most - 1) / most, step = (a->rows + passes - 1) / passes;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
   for (int row = 0; row < a->rows; row += step) {
     p.rows = a->rows - row < step ? a->rows - row : step;
     p.x = static_cast<const __nv_bfloat16*>(a->x) + row * a->x_stride;
     p.out = static_cast<uint8_t*>(a->out) + (size_t)row * a->n * (a->out_f32 ? 4 : 2);
-    int ksplit = 1;
-    while (ksplit < 8 && (bytes(ksplit, MAX_TILES / 8 + 2) > ROOM ||
-                          (p.tiles * ksplit * 2 <= 148 * 2 && p.kb >= ksplit * 2 * 2 * WARPS))) ksplit *= 2;
-    int groups = 148 * 2 / ksplit;
-    if (groups > p.tiles) groups = p.tiles;
-    if (groups < (p.tiles + MAX_TILES - 1) / MAX_TILES) groups = (p.tiles + MAX_TILES - 1) / MAX_TILES;
-    p.ksplit = ksplit; p.groups = groups;
-    p.list_blocks = bank ? ((p.tiles + groups - 1) / groups + 7) / 8 + 1 : 0;
-    const size_t smem = bytes(ksplit, p.list_blocks);
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int status = p.rows <= 8 ? (bank ? launch<1, true>(p, smem, st) : launch<1, false>(p, smem, st))
-                     : p.rows <= 16 ? (bank ? launch<2, true>(p, smem, st) : launch<2, false>(p, smem, st))
-                                    : (bank ? launch<4, true>(p, smem, st) : launch<4, false>(p, smem, st));
+    const int status = p.rows <= 8 ? (bank ? launch<1, true>(p, st) : launch<1, false>(p, st))
+                     : p.rows <= 16 ? (bank ? launch<2, true>(p, st) : launch<2, false>(p, st))
+                                    : (bank ? launch<4, true>(p, st) : launch<4, false>(p, st));
     if (status) return status;
   }
   return TW_OK;

@@ -262,6 +262,8 @@ def fp4_matvec(x, codes, scales, factor, *, prescale=None, bias=None, wr=None, w
     flat = x if x.ndim == 2 else x.reshape(-1, k)
     if flat.stride(1) != 1 or (rows > 1 and flat.stride(0) % 8) or flat.data_ptr() % 16:
         flat = flat.clone(memory_format=torch.contiguous_format)
+    if prescale is not None and prescale.data_ptr() % 16:
+        prescale = prescale.clone()
     shape = (*x.shape[:-1], n)
     if out is None:
         out = torch.empty(shape, device=dev, dtype=out_dtype)
