@@ -197,6 +197,29 @@ typedef struct TwAttentionArgs {
 size_t tw_attention_workspace(int m, int n, int hq, int hk);
 int tw_attention(const TwAttentionArgs* args, void* stream);
 
+/* ---- attention of one token over a paged cache -------------------------------------------------
+ * out[b, h] = sum_t softmax_t(scale * q[b, h] . k_t) v_t over the tokens t < lengths[s] of slot s = slots[b] (b when slots is
+ * NULL), k_t = k_pages[table[s, t / page], h / (hq / hk), t % page] (times k_scale[h / (hq / hk)]), v_t alike. An empty
+ * sequence gives zeros and lse = -inf. What lies behind a sequence's end in its last page is not used, whatever it is.
+ * Pages: [pages, hk, page, dim], rows contiguous, bf16 or (fp8) E4M3; page a power of two; dim 64 or 128; any hq / hk.
+ * A slot, length or table entry that leads outside is left out (its tokens do not count) and reported in *status. Scratch needs no
+ * initialisation; calls that may overlap need scratch of their own. Two launches. */
+typedef struct TwPagedAttentionArgs {
+  const void* q;                 /* bf16, q[b, h, :] at q + b * q_stride_batch + h * q_stride_head; even strides */
+  const void *k_pages, *v_pages;
+  const int32_t *table, *lengths, *slots; /* table [sequences, max_pages] with table_stride; lengths [sequences]; slots [batch] or NULL */
+  const float *k_scale, *v_scale;/* [hk] or NULL */
+  void* out;                     /* bf16 [batch, hq, dim] */
+  float* lse;                    /* [batch, hq] natural log of the softmax's sum, or NULL */
+  void* workspace;               /* tw_paged_attention_workspace(batch, hq, hk, dim, max_pages * page) bytes */
+  int32_t* status;               /* device word, or NULL */
+  long long q_stride_batch, q_stride_head, k_stride_page, k_stride_head, v_stride_page, v_stride_head, table_stride; /* elements */
+  float scale;
+  int32_t batch, sequences, hq, hk, dim, page, pages, max_pages, fp8;
+} TwPagedAttentionArgs;
+size_t tw_paged_attention_workspace(int batch, int hq, int hk, int dim, long long tokens);
+int tw_paged_attention(const TwPagedAttentionArgs* args, void* stream);
+
 /* ---- pointwise producers with fused tensor factor ------------------------------------------
  * Each writes its bf16 result once and, when `stats` is given, reduces max|y| in the same pass:
  * stats[0] = factor = max|y| / 2688 (1.0 for an all-zero tensor, thunderworld_fp4/_linear_kernels.py:17-19

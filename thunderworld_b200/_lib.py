@@ -59,6 +59,14 @@ class MatvecArgs(ctypes.Structure):
                [(n, _i) for n in ('rows', 'n', 'k', 'slots', 'entries', 'shared', 'dense', 'out_f32')]
 
 
+class PagedAttentionArgs(ctypes.Structure):
+    _fields_ = [(n, _vp) for n in ('q', 'k_pages', 'v_pages', 'table', 'lengths', 'slots', 'k_scale', 'v_scale', 'out', 'lse', 'workspace',
+                                   'status')] + \
+               [(n, _ll) for n in ('q_stride_batch', 'q_stride_head', 'k_stride_page', 'k_stride_head', 'v_stride_page', 'v_stride_head',
+                                   'table_stride')] + [('scale', _f)] + \
+               [(n, _i) for n in ('batch', 'sequences', 'hq', 'hk', 'dim', 'page', 'pages', 'max_pages', 'fp8')]
+
+
 _lib = None
 
 
@@ -107,6 +115,8 @@ def load():
     lib.tw_gate_residual_norm.restype = _i
     lib.tw_capture_id.argtypes = [_vp]; lib.tw_capture_id.restype = ctypes.c_ulonglong
     lib.tw_matvec.argtypes = [ctypes.POINTER(MatvecArgs), _vp]; lib.tw_matvec.restype = _i
+    lib.tw_paged_attention_workspace.argtypes = [_i] * 4 + [_ll]; lib.tw_paged_attention_workspace.restype = ctypes.c_size_t
+    lib.tw_paged_attention.argtypes = [ctypes.POINTER(PagedAttentionArgs), _vp]; lib.tw_paged_attention.restype = _i
     _lib = lib
     return lib
 
@@ -125,4 +135,5 @@ EXPORTS = ('tw_status', 'tw_abi_version', 'tw_quantize_workspace', 'tw_quantize'
            'tw_quantize_static_max_tiles', 'tw_swizzle_scales', 'tw_activation_rank', 'tw_selftest_bounded_wait',
            'tw_workspace', 'tw_fused', 'tw_fused_tile_n', 'tw_pack_rows', 'tw_select_tiles', 'tw_attention',
            'tw_attention_workspace', 'tw_activate', 'tw_rms_norm', 'tw_rms_norm_heads', 'tw_rope_heads', 'tw_gate_residual',
-           'tw_gate_residual_norm', 'tw_capture_id', 'tw_matvec')
+           'tw_gate_residual_norm', 'tw_capture_id', 'tw_matvec',
+           'tw_paged_attention_workspace', 'tw_paged_attention')

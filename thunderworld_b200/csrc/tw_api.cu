@@ -15,6 +15,8 @@ extern "C" const char* tw_status(int status) {
     case TW_ERR_TIMEOUT: return "a bounded device-side wait ran out";
     case TW_ERR_TOO_LARGE: return "size exceeds the stated maximum of this entry point";
     case TW_ERR_ARCH: return "device is not compute capability 10.x (sm_100a build)";
+    case TW_ERR_PAGE: return "a page table entry, slot or length leads outside the cache";
+    case TW_ERR_CACHE_FULL: return "the page pool or a sequence's table is full";
     default: return "unknown status";
   }
 }

@@ -22,6 +22,8 @@ enum TwStatus : int {
   TW_ERR_TIMEOUT = 8,         // a bounded device-side wait ran out (status word)
   TW_ERR_TOO_LARGE = 9,       // size beyond a stated maximum
   TW_ERR_ARCH = 10,           // device is not compute capability 10.x
+  TW_ERR_PAGE = 11,           // a page table, slot or length that leads outside the cache (status word)
+  TW_ERR_CACHE_FULL = 12,     // the pool has too few free pages, or a sequence too few entries (status word)
   TW_STATUS_COUNT
 };
 

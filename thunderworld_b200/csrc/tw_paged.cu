@@ -1,0 +1,527 @@
+// Attention of one new token per sequence over a paged key-value cache:
+//   o[b, h] = sum_t softmax_t(scale q[b, h] . k_t) v_t,  t < lengths[slot b],  k_t = k_pages[table[slot, t / page], h / G, t % page]
+// for G = hq / hk query heads per key head, head dimension 64 or 128, pages in bf16 or in E4M3 with a scale per key head.
+//
+// What bounds it is the read of the keys and values, once. The work is cut into units of 64 tokens of one (sequence, key head), in
+// that order, and the units are shared evenly by the CTAs that run beside each other, whatever the lengths (which only the device
+// knows): a CTA's run may begin and end inside a sequence, and what it has of such a one goes to the workspace, unnormalised, with
+// its maximum and sum; a second small launch joins these in their order. A call needs no zeroed state and no counter, so calls
+// on several streams, and captured ones, do not meet.
+// A warp takes 16 of a unit's tokens: it copies their rows (two units ahead) to a ring of its own, multiplies q (the group's heads,
+// padded to 16 rows) by the keys, keeps its own running maximum and sum in 32 bits, base 2, and multiplies the probabilities
+// by the values on the tensor cores (m16n8k16, 32-bit sums); warps meet only at the end of a sequence. With bf16 pages a
+// probability is two bf16 values (8 + 8 bits), so that rounding it adds nothing to the result's own rounding (an infinite value
+// then gives NaN, since the second may be zero or negative); with E4M3 pages both
+// products are in f16, which holds E4M3 exactly, and q is scaled by a power of two per head to the range of f16.
+// Tokens behind a sequence's end, and those of a table entry outside the pool (reported in the status word), are masked
+// and read as zeros, whatever lies there.
+#include <atomic>
+#include "tw_common.cuh"
+#include "../../include/twb200.h"
+
+namespace {
+
+constexpr int WARPS = 4, THREADS = WARPS * 32, UNIT = WARPS * 16;     // tokens of a unit
+constexpr int JOIN_ROWS = 4;        // query rows that a CTA's warps put together at a time
+
+struct Params {
+  const __nv_bfloat16* q; long long q_batch, q_head;
+  const uint8_t *k, *v; long long k_page, k_head, v_page, v_head;     // strides in bytes
+  const int *table; long long table_stride;
+  const int *lengths, *slots;
+  const float *k_scale, *v_scale;
+  __nv_bfloat16* out; float* lse;
+  int* prefix;                      // [batch + 1] units per key head of the sequences before
+  float *part_o, *part_ml;          // [grid][2][rows][dim], [grid][2][rows][2]
+  int* status;
+  float scale_log2;
+  int batch, sequences, hk, group, tiles, heads, page_shift, pages, max_pages, rows, grid;   // tiles of 16 query rows per key head; heads = hk * tiles
+};
+
+__device__ __forceinline__ void report(const Params& p) { if (p.status) atomicMax(p.status, (int)TW_ERR_PAGE); }
+// Tokens of batch entry b.
+__device__ __forceinline__ int tokens_of(const Params& p, int b, int& slot) {
+  slot = p.slots ? __ldg(p.slots + b) : b;
+  if (slot < 0 || slot >= p.sequences) { report(p); slot = 0; return 0; }
+  const int n = __ldg(p.lengths + slot);
+  const long long most = (long long)p.max_pages << p.page_shift;
+  if (n < 0 || n > most) { report(p); return n < 0 ? 0 : (int)most; }
+  return n;
+}
+__device__ __forceinline__ int units_of(int tokens) { return (tokens + UNIT - 1) / UNIT; }
+
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+template <bool F16>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ uint32_t e4m3_to_f16(uint32_t two) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
+  return h;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Weight of a part whose maximum is m among parts whose largest is top; nothing is left of a part without tokens.
+__device__ __forceinline__ float weight_of(float m, float top) { return m == -INFINITY ? 0.f : exp2_fast(m - top); }
+
+// Place of 16-byte chunk c of row r in a tile of rows of CHUNKS chunks: what eight lanes read at once lies in different banks.
+template <int CHUNKS> __device__ __forceinline__ int swizzled(int c, int r) { return CHUNKS == 4 ? c ^ (r >> 1 & 3) : c ^ (r & 7); }
+
+// Where a CTA is in its run of units.
+struct Cursor {
+  int unit, b, h, tile, units, tokens, slot;       // tile: of the sequence's `units`
+};
+
+template <int D, bool FP8>
+__global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __grid_constant__ Params p) {
+  constexpr int ROW = D * (FP8 ? 1 : 2), CHUNKS = ROW / 16, TILE = 16 * ROW;      // bytes of a row, of 16 rows
+  constexpr int STAGES = 2;
+  extern __shared__ __align__(128) uint8_t dynamic[];                             // [WARPS][STAGES][K, V][16 rows]
+  __shared__ float gather[WARPS * JOIN_ROWS * D];
+  __shared__ float part_m[WARPS][16], part_l[WARPS][16];
+  __shared__ int sums[WARPS + 1], start_b, start_offset;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+
+  // ---- this CTA's run: the lengths' prefix sums, in units -----------------------------------------------------------
+  const int per = (p.batch + THREADS - 1) / THREADS, first_b = min(threadIdx.x * per, p.batch), last_b = min(first_b + per, p.batch);
+  int mine = 0, slot_unused;
+  for (int b = first_b; b < last_b; ++b) mine += units_of(tokens_of(p, b, slot_unused));
+  int before = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) { const int x = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += x; }
+  if (lane == 31) sums[warp] = before;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) { if (w == warp) before += total - mine; total += sums[w]; }
+  const long long all = (long long)total * p.heads, owners = min(all, (long long)p.grid);     // every owner has a unit at least
+  const long long unit0 = blockIdx.x < owners ? all * blockIdx.x / owners : 0, unit1 = blockIdx.x < owners ? all * (blockIdx.x + 1) / owners : 0;
+  {
+    int at = before;
+    for (int b = first_b; b < last_b; ++b) {
+      const int n = units_of(tokens_of(p, b, slot_unused));
+      if (blockIdx.x == 0) p.prefix[b] = at;
+      if ((long long)at * p.heads <= unit0 && unit0 < (long long)(at + n) * p.heads) { start_b = b; start_offset = (int)(unit0 - (long long)at * p.heads); }
+      at += n;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.prefix[p.batch] = total;
+  }
+  __syncthreads();
+  if (unit0 >= unit1) return;
+  const int count = (int)(unit1 - unit0);
+
+  auto enter = [&](Cursor& c) { c.tokens = tokens_of(p, c.b, c.slot); c.units = units_of(c.tokens); };
+  auto begin = [&](Cursor& c) {
+    c.unit = 0;
+    c.b = start_b;
+    enter(c);
+    c.h = start_offset / c.units;
+    c.tile = start_offset - c.h * c.units;
+  };
+  auto advance = [&](Cursor& c) {
+    ++c.unit;
+    if (++c.tile < c.units || c.unit >= count) return;
+    c.tile = 0;
+    if (++c.h < p.heads) return;
+    c.h = 0;
+    do { ++c.b; enter(c); } while (c.units == 0);
+  };
+
+  // ---- copies: 16 tokens' rows of K and of V to the warp's ring ---------------------------------------------
+  const uint32_t ring = tw::smem_u32(dynamic) + warp * STAGES * 2 * TILE;
+  constexpr int LANES = CHUNKS, STEP = 32 / LANES, COPIES = 16 / STEP;            // lanes per row, rows per instruction
+  const int copy_row = lane / LANES, copy_chunk = lane % LANES;
+  Cursor in;
+  begin(in);
+  uint32_t masks[STAGES];              // tokens of a stage that count
+  auto fetch = [&](int stage) {
+    uint32_t mask = 0;
+    const int t0 = in.tile * UNIT + warp * 16;
+    if (in.unit < count && t0 < in.tokens) {
+      const int live = min(in.tokens - t0, 16), kv = in.h / p.tiles;
+      const int* entries = p.table + in.slot * p.table_stride;
+      const uint32_t to = ring + stage * 2 * TILE;
+      const long long k_at = kv * p.k_head, v_at = kv * p.v_head;
+      int page = -1;
+      if (p.page_shift >= 4) {         // the 16 tokens lie in one page
+        page = __ldg(entries + (t0 >> p.page_shift));
+        if (page < 0 || page >= p.pages) { if (lane == 0) report(p); } else mask = 0xffffu >> (16 - live);
+      }
+#pragma unroll
+      for (int i = 0; i < COPIES; ++i) {
+        const int r = i * STEP + copy_row, token = t0 + r;
+        bool valid = r < live;
+        if (p.page_shift < 4) {
+          page = valid ? __ldg(entries + (token >> p.page_shift)) : -1;
+          if (valid && (page < 0 || page >= p.pages)) { report(p); valid = false; }
+          // one bit per row, from the first lane of each row
+          const uint32_t votes = __ballot_sync(0xffffffffu, valid);
+#pragma unroll
+          for (int j = 0; j < STEP; ++j) mask |= (votes >> (j * LANES) & 1u) << (i * STEP + j);
+        } else {
+          valid = valid && mask;
+        }
+        const long long row = (long long)(token & ((1 << p.page_shift) - 1)) * ROW + copy_chunk * 16;
+        const uint32_t at = r * ROW + swizzled<CHUNKS>(copy_chunk, r) * 16;
+        const uint8_t* k = valid ? p.k + page * p.k_page + k_at + row : p.k;
+        const uint8_t* v = valid ? p.v + page * p.v_page + v_at + row : p.v;
+        copy16(to + at, k, valid ? 16 : 0);
+        copy16(to + TILE + at, v, valid ? 16 : 0);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    masks[stage] = mask;
+    if (in.unit < count) advance(in);
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s) fetch(s);
+
+  // ---- products -----------------------------------------------------------------------------------------------------
+  uint32_t q[D / 16][4];               // A fragments; with E4M3 pages lane t holds channels 4 t ... 4 t + 3 of each 16
+  float o[D / 8][4], m[2], l[2], score_scale[2];
+  Cursor at;
+  begin(at);
+  bool first_segment = true;
+  bool fresh = true;
+  const bool begins_inside = at.tile != 0;
+  while (at.unit < count) {
+#pragma unroll
+    for (int stage = 0; stage < STAGES; ++stage) {
+      if (at.unit >= count) break;
+      if (fresh) {
+        fresh = false;
+        const int kv = at.h / p.tiles, row0 = (at.h - kv * p.tiles) * 16;
+        const __nv_bfloat16* base = p.q + at.b * p.q_batch + (long long)(kv * p.group + row0) * p.q_head;
+        const bool low = row0 + g < p.group, high = row0 + g + 8 < p.group;
+        const __nv_bfloat16 *r0 = base + g * p.q_head, *r1 = base + (g + 8) * p.q_head;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+          const int c = FP8 ? j * 16 + t * 4 : j * 16 + t * 2, d = FP8 ? 2 : 8;
+          q[j][0] = low ? __ldg(reinterpret_cast<const uint32_t*>(r0 + c)) : 0u;
+          q[j][1] = high ? __ldg(reinterpret_cast<const uint32_t*>(r1 + c)) : 0u;
+          q[j][2] = low ? __ldg(reinterpret_cast<const uint32_t*>(r0 + c + d)) : 0u;
+          q[j][3] = high ? __ldg(reinterpret_cast<const uint32_t*>(r1 + c + d)) : 0u;
+        }
+        const float k_scale = p.k_scale ? __ldg(p.k_scale + kv) : 1.f;
+        score_scale[0] = score_scale[1] = p.scale_log2 * k_scale;
+        if (FP8) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {                   // rows g and g + 8 to the range of f16, as the largest finite value says
+            unsigned top = 0;
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t w = q[j][h + 2 * i], lo = (w & 0x7fffu) << 16, hi = w & 0x7fff0000u;
+                top = max(top, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));
+              }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int shift = top ? min(14 - ((int)(top >> 23) - 127), 126) : 0;
+            const float up = __uint_as_float((unsigned)(127 + shift) << 23);
+            score_scale[h] *= __uint_as_float((unsigned)(127 - shift) << 23);
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t w = q[j][h + 2 * i];
+                q[j][h + 2 * i] = pack_f16(tw::bf16_bits_to_float(w & 0xffffu) * up, tw::bf16_bits_to_float(w >> 16) * up);
+              }
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
+      }
+
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+      __syncwarp();
+      const uint32_t mask = masks[stage], keys = ring + stage * 2 * TILE, values = keys + TILE;
+      if (mask) {
+        float s[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+          if (FP8) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              uint32_t w;
+              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(keys + (n * 8 + g) * ROW + swizzled<CHUNKS>(j, n * 8 + g) * 16 + t * 4) : "memory");
+              mma<true>(s[n], q[j], e4m3_to_f16(w & 0xffffu), e4m3_to_f16(w >> 16));
+            }
+          } else {
+            // matrices: tokens 0-7 and 8-15 (lane / 16) of channels 16 j ... + 7 and + 8 ... + 15 (lane / 8 % 2)
+            uint32_t b[4];
+            const int r = (lane & 7) + (lane >> 4) * 8, c = j * 2 + (lane >> 3 & 1);
+            ldsm4(b, keys + r * ROW + swizzled<CHUNKS>(c, r) * 16);
+            mma<false>(s[0], q[j], b[0], b[1]);
+            mma<false>(s[1], q[j], b[2], b[3]);
+          }
+        }
+        // scores in base 2; row g in elements 0 and 1, row g + 8 in 2 and 3; tokens 8 n + 2 t and the next
+        float top[2] = {m[0], m[1]};
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[n][i] *= score_scale[i >> 1];
+            if (!(mask >> (n * 8 + t * 2 + (i & 1)) & 1u)) s[n][i] = -INFINITY;
+            top[i >> 1] = fmaxf(top[i >> 1], s[n][i]);
+          }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+          top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+        }
+        if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+          const float a0 = weight_of(m[0], top[0]), a1 = weight_of(m[1], top[1]);
+          m[0] = top[0];
+          m[1] = top[1];
+          l[0] *= a0;
+          l[1] *= a1;
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) { o[n][0] *= a0; o[n][1] *= a0; o[n][2] *= a1; o[n][3] *= a1; }
+        }
+        const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[n][i] = exp2_fast(s[n][i] - ref[i >> 1]);
+            l[i >> 1] += s[n][i];
+          }
+        uint32_t hi[4], lo[4];         // probabilities as an A fragment: rows g, g + 8; tokens 2 t, 2 t + 8
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = s[i >> 1][(i & 1) * 2], y = s[i >> 1][(i & 1) * 2 + 1];
+          if (FP8) {
+            hi[i] = pack_f16(x, y);
+          } else {
+            hi[i] = pack_bf16(x, y);
+            lo[i] = pack_bf16(x - tw::bf16_bits_to_float(hi[i] & 0xffffu), y - tw::bf16_bits_to_float(hi[i] >> 16));
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < CHUNKS / 2; ++c) {
+          // matrices: tokens 0-7 and 8-15 (lane / 8 % 2) of chunks 2 c and 2 c + 1 (lane / 16)
+          uint32_t b[4];
+          const int r = lane & 15, ch = c * 2 + (lane >> 4);
+          ldsm4_trans(b, values + r * ROW + swizzled<CHUNKS>(ch, r) * 16);
+          if (FP8) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {                 // a chunk's 16 channels: the even ones and the odd ones
+              const uint32_t x = b[2 * h], y = b[2 * h + 1];
+              mma<true>(o[c * 4 + h * 2], hi, e4m3_to_f16(__byte_perm(x, 0, 0x4420)), e4m3_to_f16(__byte_perm(y, 0, 0x4420)));
+              mma<true>(o[c * 4 + h * 2 + 1], hi, e4m3_to_f16(__byte_perm(x, 0, 0x4431)), e4m3_to_f16(__byte_perm(y, 0, 0x4431)));
+            }
+          } else {
+            mma<false>(o[c * 2], hi, b[0], b[1]);
+            mma<false>(o[c * 2], lo, b[0], b[1]);
+            mma<false>(o[c * 2 + 1], hi, b[2], b[3]);
+            mma<false>(o[c * 2 + 1], lo, b[2], b[3]);
+          }
+        }
+      }
+      __syncwarp();
+      fetch(stage);
+
+      const bool last = at.tile + 1 == at.units;
+      if (last || at.unit + 1 == count) {
+        // ---- the sequence's, or the run's, end: the warps' parts together -------------------------------------------
+        const bool whole = last && !(first_segment && begins_inside);
+        const int kv = at.h / p.tiles, row0 = (at.h - kv * p.tiles) * 16, rows = min(p.group - row0, 16);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+          l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+          if (t == 0) { part_m[warp][g + 8 * h] = m[h]; part_l[warp][g + 8 * h] = l[h]; }
+        }
+        const float v_scale = p.v_scale ? __ldg(p.v_scale + kv) : 1.f;
+        for (int r0 = 0; r0 < rows; r0 += JOIN_ROWS) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = g + 8 * h - r0;
+            if (r >= 0 && r < JOIN_ROWS) {
+              float* to = gather + (warp * JOIN_ROWS + r) * D;
+#pragma unroll
+              for (int n = 0; n < D / 8; ++n) {
+                // E4M3: tiles 2 c and 2 c + 1 hold the even and odd channels of chunk c
+                const int d0 = FP8 ? (n >> 1) * 16 + t * 4 + (n & 1) : n * 8 + t * 2, d1 = d0 + (FP8 ? 2 : 1);
+                to[d0] = o[n][2 * h];
+                to[d1] = o[n][2 * h + 1];
+              }
+            }
+          }
+          __syncthreads();
+          for (int e = threadIdx.x; e < JOIN_ROWS * D; e += THREADS) {
+            const int r = r0 + e / D, d = e % D;
+            if (r >= rows) break;
+            float top = part_m[0][r], sum = 0.f, y = 0.f;
+#pragma unroll
+            for (int w = 1; w < WARPS; ++w) top = fmaxf(top, part_m[w][r]);
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+              const float a = weight_of(part_m[w][r], top);
+              sum += a * part_l[w][r];
+              y += a * gather[(w * JOIN_ROWS + r - r0) * D + d];
+            }
+            if (whole) {
+              const long long head = (long long)at.b * p.hk * p.group + kv * p.group + row0 + r;
+              p.out[head * D + d] = __float2bfloat16_rn(sum == 0.f ? 0.f : y * v_scale / sum);
+              if (p.lse && d == 0) p.lse[head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945f;
+            } else {
+              const long long slot = ((long long)blockIdx.x * 2 + (first_segment ? 0 : 1)) * p.rows + r;
+              p.part_o[slot * D + d] = y;
+              if (d == 0) { p.part_ml[slot * 2] = top; p.part_ml[slot * 2 + 1] = sum; }
+            }
+          }
+          __syncthreads();
+        }
+        first_segment = false;
+        fresh = true;
+      }
+      advance(at);
+    }
+  }
+}
+
+// Joins what several CTAs have of one (sequence, head tile), and writes the rows of empty sequences.
+template <int D>
+__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ Params p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");       // the parts are written
+  const int b = blockIdx.x / p.heads, h = blockIdx.x - b * p.heads, kv = h / p.tiles, row0 = (h - kv * p.tiles) * 16, rows = min(p.group - row0, 16);
+  const int from = p.prefix[b], units = p.prefix[b + 1] - from;
+  const long long all = (long long)p.prefix[p.batch] * p.heads, begin = (long long)from * p.heads + (long long)h * units, end = begin + units;
+  const long long head0 = (long long)b * p.hk * p.group + kv * p.group + row0;
+  if (units == 0) {
+    for (int e = threadIdx.x; e < rows * D; e += 128) p.out[head0 * D + e] = __float2bfloat16_rn(0.f);
+    if (p.lse) for (int r = threadIdx.x; r < rows; r += 128) p.lse[head0 + r] = -INFINITY;
+    return;
+  }
+  // CTA c has the units [all c / owners, all (c + 1) / owners): that of unit u is the last c with all c / owners <= u
+  const long long owners = min(all, (long long)p.grid);
+  auto owner = [&](long long u) { return (int)(((u + 1) * owners + all - 1) / all) - 1; };
+  const int c0 = owner(begin), c1 = owner(end - 1);
+  if (c0 == c1) return;
+  const int slot0 = all * c0 / owners == begin ? 0 : 1;    // a CTA's first sequence is its part 0
+  const float v_scale = p.v_scale ? __ldg(p.v_scale + kv) : 1.f;
+  for (int e = threadIdx.x; e < rows * D; e += 128) {
+    const int r = e / D, d = e - r * D;
+    float top = -INFINITY, sum = 0.f, y = 0.f;
+    for (int c = c0; c <= c1; ++c) top = fmaxf(top, p.part_ml[(((long long)c * 2 + (c == c0 ? slot0 : 0)) * p.rows + r) * 2]);
+    for (int c = c0; c <= c1; ++c) {
+      const long long slot = ((long long)c * 2 + (c == c0 ? slot0 : 0)) * p.rows + r;
+      const float a = weight_of(p.part_ml[slot * 2], top);
+      sum += a * p.part_ml[slot * 2 + 1];
+      y += a * p.part_o[slot * D + d];
+    }
+    p.out[(head0 + r) * D + d] = __float2bfloat16_rn(sum == 0.f ? 0.f : y * v_scale / sum);
+    if (p.lse && d == 0) p.lse[head0 + r] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945f;
+  }
+}
+
+// CTAs that run beside each other, for units of which there are at most `most`.
+int grid_of(long long most) { const long long fit = 148 * 3; return (int)(most < 1 ? 1 : most < fit ? most : fit); }
+int grid_of(int batch, int hq, int hk, long long tokens) {
+  const long long tiles = (hq / hk + 15) / 16;
+  return grid_of((long long)batch * hk * tiles * ((tokens + UNIT - 1) / UNIT));
+}
+size_t prefix_bytes(int batch) { return ((size_t)(batch + 1) * 4 + 15) / 16 * 16; }
+int part_rows(int hq, int hk) { return hq / hk < 16 ? hq / hk : 16; }
+
+template <int D, bool FP8>
+int launch(const Params& p, cudaStream_t stream) {
+  constexpr int SMEM = WARPS * 2 * 2 * 16 * D * (FP8 ? 1 : 2);
+  static std::atomic<bool> configured[64];            // the shared-memory opt-in is a per-device attribute of the function
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) { (void)cudaGetLastError(); return TW_ERR_LAUNCH; }
+  if (device >= 64 || !configured[device].load(std::memory_order_relaxed)) {
+    if (cudaFuncSetAttribute(paged_attention_kernel<D, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return TW_ERR_LAUNCH;
+    }
+    if (device < 64) configured[device].store(true, std::memory_order_relaxed);
+  }
+  paged_attention_kernel<D, FP8><<<p.grid, THREADS, SMEM, stream>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return TW_ERR_LAUNCH;
+  // the join's launch overlaps the end of the first kernel; it waits for it before it reads anything
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(p.batch * p.heads);
+  config.blockDim = dim3(128);
+  config.stream = stream;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  if (cudaLaunchKernelEx(&config, paged_join_kernel<D>, p) != cudaSuccess) { (void)cudaGetLastError(); return TW_ERR_LAUNCH; }
+  return TW_OK;
+}
+
+bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
+
+}  // namespace
+
+extern "C" size_t tw_paged_attention_workspace(int batch, int hq, int hk, int dim, long long tokens) {
+  if (batch <= 0 || hk <= 0 || hq <= 0 || hq % hk || dim <= 0 || tokens < 0) return 0;
+  return prefix_bytes(batch) + (size_t)grid_of(batch, hq, hk, tokens) * 2 * part_rows(hq, hk) * (dim + 2) * 4;
+}
+
+extern "C" int tw_paged_attention(const TwPagedAttentionArgs* a, void* stream) {
+  if (!a || !a->q || !a->k_pages || !a->v_pages || !a->table || !a->lengths || !a->out || !a->workspace || a->batch <= 0 || a->sequences <= 0 ||
+      a->hq <= 0 || a->hk <= 0 || a->hq % a->hk || a->page <= 0 || a->pages <= 0 || a->max_pages <= 0)
+    return TW_ERR_ARGUMENT;
+  if ((a->dim != 64 && a->dim != 128) || (a->page & (a->page - 1))) return TW_ERR_SHAPE;
+  const long long tokens = (long long)a->max_pages * a->page;
+  const int tiles = (a->hq / a->hk + 15) / 16, heads = a->hk * tiles;
+  if (a->page > (1 << 20) || tokens > (1LL << 30) || (long long)a->batch * heads > (1 << 30) ||
+      (long long)a->batch * ((tokens + UNIT - 1) / UNIT) > (1LL << 31) - 1)
+    return TW_ERR_TOO_LARGE;
+  const int bytes = a->fp8 ? 1 : 2;
+  if (misaligned(a->q, 4) || (a->q_stride_batch | a->q_stride_head) & 1 || misaligned(a->k_pages, 16) || misaligned(a->v_pages, 16) ||
+      ((a->k_stride_page | a->k_stride_head | a->v_stride_page | a->v_stride_head) * bytes) % 16 || misaligned(a->workspace, 16) ||
+      misaligned(a->out, 2) || misaligned(a->table, 4) || misaligned(a->lengths, 4))
+    return TW_ERR_ALIGNMENT;
+  Params p = {};
+  p.q = static_cast<const __nv_bfloat16*>(a->q); p.q_batch = a->q_stride_batch; p.q_head = a->q_stride_head;
+  p.k = static_cast<const uint8_t*>(a->k_pages); p.v = static_cast<const uint8_t*>(a->v_pages);
+  p.k_page = a->k_stride_page * bytes; p.k_head = a->k_stride_head * bytes;
+  p.v_page = a->v_stride_page * bytes; p.v_head = a->v_stride_head * bytes;
+  p.table = a->table; p.table_stride = a->table_stride; p.lengths = a->lengths; p.slots = a->slots;
+  p.k_scale = a->k_scale; p.v_scale = a->v_scale;
+  p.out = static_cast<__nv_bfloat16*>(a->out); p.lse = a->lse; p.status = a->status;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.batch = a->batch; p.sequences = a->sequences; p.hk = a->hk; p.group = a->hq / a->hk; p.tiles = tiles; p.heads = heads;
+  p.pages = a->pages; p.max_pages = a->max_pages; p.rows = part_rows(a->hq, a->hk); p.grid = grid_of(a->batch, a->hq, a->hk, tokens);
+  while ((1 << p.page_shift) < a->page) ++p.page_shift;
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  p.prefix = reinterpret_cast<int*>(ws);
+  p.part_ml = reinterpret_cast<float*>(ws + prefix_bytes(a->batch));
+  p.part_o = p.part_ml + (size_t)p.grid * 2 * p.rows * 2;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a->dim == 128) return a->fp8 ? launch<128, true>(p, st) : launch<128, false>(p, st);
+  return a->fp8 ? launch<64, true>(p, st) : launch<64, false>(p, st);
+}

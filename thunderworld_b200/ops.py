@@ -278,12 +278,111 @@ def fp4_matvec(x, codes, scales, factor, *, prescale=None, bias=None, wr=None, w
     return out
 
 
-STATUS_KEYS = {'g': 0, 'a': 0, 'q': 8}   # workspace -> byte offset of its device status word: fused GEMM, attention, quantizer
+# ---- paged key-value cache --------------------------------------------------------------------------
+def _cache_status(device):
+    """The device word that the paged operators report in (device_status reads it)."""
+    word = _workspaces.get((device, 'c'))
+    if word is None:
+        word = _workspace(device, 256, 'c')
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(device).synchronize()       # zeroed before another stream's call may write it
+    return word
+
+
+def _check_pages(k_pages, v_pages):
+    """(pages, kv heads, page, dim, fp8) of the two halves of a pool; raises where they are not pages."""
+    if k_pages.ndim != 4 or k_pages.shape != v_pages.shape or not k_pages.numel():
+        raise ValueError('k_pages and v_pages must be [pages, kv_heads, page, dim] alike')
+    if k_pages.dtype is not v_pages.dtype or (k_pages.dtype is not torch.bfloat16 and k_pages.dtype is not torch.float8_e4m3fn):
+        raise ValueError('pages must be bfloat16 or float8_e4m3fn')
+    pages, hk, page, dim = k_pages.shape
+    if dim != 64 and dim != 128:
+        raise ValueError('head dimension must be 64 or 128')
+    if page & (page - 1):
+        raise ValueError('tokens per page must be a power of two')
+    for t in (k_pages, v_pages):
+        if t.stride(3) != 1 or (page > 1 and t.stride(2) != dim):
+            raise ValueError('the rows of a page must lie one behind the other')
+    if not k_pages.is_cuda or v_pages.device != k_pages.device:
+        raise ValueError('pages must be on one CUDA device')
+    return pages, hk, page, dim, k_pages.dtype is torch.float8_e4m3fn
+
+
+def _check_int32(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and (t.dtype is not torch.int32 or t.device != device or t.ndim != 1 or (t.numel() > 1 and t.stride(0) != 1)):
+            raise ValueError(f'{name} must be contiguous int32 on the device of the pages')
+
+
+def _check_table(device, table, lengths):
+    if table.ndim != 2 or table.dtype is not torch.int32 or table.device != device or not table.numel() or table.stride(1) != 1:
+        raise ValueError('table must be int32 [sequences, pages per sequence] with contiguous rows, on the device of the pages')
+    _check_int32(device, lengths=lengths)
+    if lengths.numel() != table.shape[0]:
+        raise ValueError('lengths must hold one entry per row of table')
+
+
+def _check_scales(device, hk, k_scale, v_scale, fp8):
+    for name, t in (('k_scale', k_scale), ('v_scale', v_scale)):
+        if t is not None:
+            if not fp8:
+                raise ValueError('scales come with float8_e4m3fn pages')
+            if t.dtype is not torch.float32 or t.device != device or tuple(t.shape) != (hk,) or not t.is_contiguous():
+                raise ValueError(f'{name} must be contiguous float32 [kv_heads] on the device of the pages')
+
+
+def paged_attention(q, k_pages, v_pages, table, lengths, *, slots=None, scale=None, k_scale=None, v_scale=None, return_lse=False, out=None):
+    """Attention of one new token per sequence over a paged cache: q bf16 [batch, heads, dim], row b over the lengths[s] tokens of
+    slot s = slots[b] (b by default), token t at k_pages[table[s, t // page], h // (heads / kv_heads), t % page].
+
+    Pages [pages, kv_heads, page, dim] in bf16 or float8_e4m3fn (times k_scale / v_scale [kv_heads]), page a power of two, dim 64 or
+    128; table int32 [sequences, pages per sequence], lengths int32 [sequences], slots int32 [batch], all read on the device:
+    no host synchronisation. scale defaults to dim ** -0.5. Returns bf16 [batch, heads, dim], with return_lse also the float32
+    natural log of each softmax's sum (-inf and zeros for an empty sequence). Sums are 32 bits wide. Slots, lengths and table entries
+    that lead outside are left out and reported by device_status()."""
+    pages, hk, page, dim, fp8 = _check_pages(k_pages, v_pages)
+    dev = k_pages.device
+    if q.ndim != 3 or q.dtype is not torch.bfloat16 or q.device != dev or q.shape[2] != dim or q.stride(2) != 1:
+        raise ValueError('q must be BF16 [batch, heads, dim] with contiguous rows, on the device of the pages')
+    batch, hq = q.shape[0], q.shape[1]
+    if not batch or not hq or hq % hk:
+        raise ValueError('a nonempty batch and a whole number of heads per kv head are required')
+    _check_table(dev, table, lengths)
+    _check_int32(dev, slots=slots)
+    if (batch if slots is None else slots.numel()) != batch or (slots is None and batch > table.shape[0]):
+        raise ValueError('slots must name one sequence per row of q')
+    _check_scales(dev, hk, k_scale, v_scale, fp8)
+    if torch.is_grad_enabled() and q.requires_grad:
+        raise RuntimeError('paged_attention is inference-only; use torch.inference_mode()')
+    require_sm100(dev)
+    if q.data_ptr() % 4 or q.stride(0) % 2 or q.stride(1) % 2:
+        q = q.contiguous() if not q.is_contiguous() else q.clone()
+    shape = (batch, hq, dim)
+    if out is None:
+        out = torch.empty(shape, device=dev, dtype=torch.bfloat16)
+    elif tuple(out.shape) != shape or out.dtype is not torch.bfloat16 or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f'out must be contiguous BF16 {shape} on the device of the pages')
+    lse = torch.empty((batch, hq), device=dev, dtype=torch.float32) if return_lse else None
+    lib = _lib.load()
+    with _device(dev):
+        # scratch of the call's own: calls on several streams, and captured ones, do not share it
+        scratch = torch.empty(lib.tw_paged_attention_workspace(batch, hq, hk, dim, table.shape[1] * page), device=dev, dtype=torch.uint8)
+        args = _lib.PagedAttentionArgs(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lengths.data_ptr(), _ptr(slots), _ptr(k_scale), _ptr(v_scale),
+            out.data_ptr(), _ptr(lse), scratch.data_ptr(), _cache_status(dev).data_ptr(), q.stride(0), q.stride(1), k_pages.stride(0),
+            k_pages.stride(1), v_pages.stride(0), v_pages.stride(1), table.stride(0), dim ** -.5 if scale is None else float(scale), batch,
+            table.shape[0], hq, hk, dim, page, pages, table.shape[1], int(fp8))
+        _lib.check(lib.tw_paged_attention(ctypes.byref(args), _stream(dev)))
+    return (out, lse) if return_lse else out
+
+
+STATUS_KEYS = {'g': 0, 'a': 0, 'q': 8, 'c': 0}   # workspace -> byte offset of its device status word: fused GEMM, attention, quantizer, paged cache
 
 
 def device_status(device=None):
     """Worst status word any kernel of this device wrote on a bounded-wait timeout (0 = none); synchronises.
-    Covers the fused GEMM, the attention kernel and the single-pass quantizer's grid barrier: each writes into its own workspace."""
+    Covers the fused GEMM, the attention kernel and the single-pass quantizer's grid barrier: each writes into its own workspace;
+    and what the operators of the paged cache found and left out (an entry outside the cache, a full pool)."""
     dev = torch.device('cuda', torch.cuda.current_device()) if device is None else torch.device(device)
     if dev.index is None:
         dev = torch.device('cuda', torch.cuda.current_device())
