@@ -31,7 +31,7 @@ struct Params {
   const int *lengths, *slots;
   const float *k_scale, *v_scale;
   __nv_bfloat16* out; float* lse;
-  int* prefix;                      // [batch + 1] units per key head of the sequences before
+  int4* starts;                     // [grid] batch entry, head, tile and number of tiles where a CTA's run begins; batch -1: no run
   float *part_o, *part_ml;          // [grid][2][rows][dim], [grid][2][rows][2]
   int* status;
   float scale_log2;
@@ -121,14 +121,22 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
     int at = before;
     for (int b = first_b; b < last_b; ++b) {
       const int n = units_of(tokens_of(p, b, slot_unused));
-      if (blockIdx.x == 0) p.prefix[b] = at;
       if ((long long)at * p.heads <= unit0 && unit0 < (long long)(at + n) * p.heads) { start_b = b; start_offset = (int)(unit0 - (long long)at * p.heads); }
       at += n;
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.prefix[p.batch] = total;
+    // rows of empty sequences, dealt out over the CTAs
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+      if (tokens_of(p, b, slot_unused)) continue;
+      const long long head0 = (long long)b * p.hk * p.group, heads = p.hk * p.group;
+      for (long long e = threadIdx.x; e < heads * D; e += THREADS) p.out[head0 * D + e] = __float2bfloat16_rn(0.f);
+      if (p.lse) for (int e = threadIdx.x; e < heads; e += THREADS) p.lse[head0 + e] = -INFINITY;
+    }
   }
   __syncthreads();
-  if (unit0 >= unit1) return;
+  if (unit0 >= unit1) {
+    if (threadIdx.x == 0) p.starts[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    return;
+  }
   const int count = (int)(unit1 - unit0);
 
   auto enter = [&](Cursor& c) { c.tokens = tokens_of(p, c.b, c.slot); c.units = units_of(c.tokens); };
@@ -154,6 +162,7 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
   const int copy_row = lane / LANES, copy_chunk = lane % LANES;
   Cursor in;
   begin(in);
+  if (threadIdx.x == 0) p.starts[blockIdx.x] = make_int4(in.b, in.h, in.tile, in.units);
   uint32_t masks[STAGES];              // tokens of a stage that count
   auto fetch = [&](int stage) {
     uint32_t mask = 0;
@@ -408,39 +417,67 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
   }
 }
 
-// Joins what several CTAs have of one (sequence, head tile), and writes the rows of empty sequences.
+// Joins what several CTAs have of one (sequence, head tile): a block per border between two CTAs' runs and query row, which works
+// if its border is the first one inside the sequence.
+constexpr int JOIN_THREADS = 256;
 template <int D>
-__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const __grid_constant__ Params p) {
+  extern __shared__ float weights[];                       // [grid]
+  __shared__ float reduce[JOIN_THREADS / 32], sums[JOIN_THREADS / D][D];
   asm volatile("griddepcontrol.wait;" ::: "memory");       // the parts are written
-  const int b = blockIdx.x / p.heads, h = blockIdx.x - b * p.heads, kv = h / p.tiles, row0 = (h - kv * p.tiles) * 16, rows = min(p.group - row0, 16);
-  const int from = p.prefix[b], units = p.prefix[b + 1] - from;
-  const long long all = (long long)p.prefix[p.batch] * p.heads, begin = (long long)from * p.heads + (long long)h * units, end = begin + units;
-  const long long head0 = (long long)b * p.hk * p.group + kv * p.group + row0;
-  if (units == 0) {
-    for (int e = threadIdx.x; e < rows * D; e += 128) p.out[head0 * D + e] = __float2bfloat16_rn(0.f);
-    if (p.lse) for (int r = threadIdx.x; r < rows; r += 128) p.lse[head0 + r] = -INFINITY;
-    return;
+  const int border = blockIdx.x + 1, r = blockIdx.y;
+  const int4 here = p.starts[border], before = p.starts[border - 1];
+  if (here.x < 0 || here.z == 0) return;                   // no run, or one that begins with its sequence
+  const bool same = before.x == here.x && before.y == here.y;
+  if (same && before.z > 0) return;                        // the run before begins inside the same sequence
+  const int kv = here.y / p.tiles, row0 = (here.y - kv * p.tiles) * 16;
+  if (row0 + r >= p.group) return;
+  // parts: the last of the run before (its first, if that begins with this sequence), and the first of every run that begins in it
+  __shared__ int after;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) after = p.grid;
+  __syncthreads();
+  for (int c = border + threadIdx.x; c < p.grid; c += JOIN_THREADS) {
+    const int4 x = p.starts[c];
+    if (x.x != here.x || x.y != here.y) { atomicMin(&after, c); break; }
   }
-  // CTA c has the units [all c / owners, all (c + 1) / owners): that of unit u is the last c with all c / owners <= u
-  const long long owners = min(all, (long long)p.grid);
-  auto owner = [&](long long u) { return (int)(((u + 1) * owners + all - 1) / all) - 1; };
-  const int c0 = owner(begin), c1 = owner(end - 1);
-  if (c0 == c1) return;
-  const int slot0 = all * c0 / owners == begin ? 0 : 1;    // a CTA's first sequence is its part 0
+  __syncthreads();
+  const int parts = after - border + 1;
+  auto slot_of = [&](int i) { return ((long long)(border - 1 + i) * 2 + (i == 0 && !same ? 1 : 0)) * p.rows + r; };
+  float top = -INFINITY;
+  for (int i = threadIdx.x; i < parts; i += JOIN_THREADS) { weights[i] = p.part_ml[slot_of(i) * 2]; top = fmaxf(top, weights[i]); }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) reduce[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < JOIN_THREADS / 32; ++w) top = fmaxf(top, reduce[w]);
+  __syncthreads();
+  float sum = 0.f;
+  for (int i = threadIdx.x; i < parts; i += JOIN_THREADS) {
+    weights[i] = weight_of(weights[i], top);
+    sum += weights[i] * p.part_ml[slot_of(i) * 2 + 1];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) reduce[warp] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < JOIN_THREADS / 32; ++w) sum += reduce[w];
+  const int d = threadIdx.x % D, share = threadIdx.x / D;
+  float y = 0.f;
+#pragma unroll 8
+  for (int i = share; i < parts; i += JOIN_THREADS / D) y += weights[i] * p.part_o[slot_of(i) * D + d];
+  sums[share][d] = y;
+  __syncthreads();
+  if (share) return;
+#pragma unroll
+  for (int w = 1; w < JOIN_THREADS / D; ++w) y += sums[w][d];
+  const long long head = (long long)here.x * p.hk * p.group + kv * p.group + row0 + r;
   const float v_scale = p.v_scale ? __ldg(p.v_scale + kv) : 1.f;
-  for (int e = threadIdx.x; e < rows * D; e += 128) {
-    const int r = e / D, d = e - r * D;
-    float top = -INFINITY, sum = 0.f, y = 0.f;
-    for (int c = c0; c <= c1; ++c) top = fmaxf(top, p.part_ml[(((long long)c * 2 + (c == c0 ? slot0 : 0)) * p.rows + r) * 2]);
-    for (int c = c0; c <= c1; ++c) {
-      const long long slot = ((long long)c * 2 + (c == c0 ? slot0 : 0)) * p.rows + r;
-      const float a = weight_of(p.part_ml[slot * 2], top);
-      sum += a * p.part_ml[slot * 2 + 1];
-      y += a * p.part_o[slot * D + d];
-    }
-    p.out[(head0 + r) * D + d] = __float2bfloat16_rn(sum == 0.f ? 0.f : y * v_scale / sum);
-    if (p.lse && d == 0) p.lse[head0 + r] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945f;
-  }
+  p.out[head * D + d] = __float2bfloat16_rn(sum == 0.f ? 0.f : y * v_scale / sum);
+  if (p.lse && d == 0) p.lse[head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945f;
 }
 
 // CTAs that run beside each other, for units of which there are at most `most`.
@@ -449,7 +486,6 @@ int grid_of(int batch, int hq, int hk, long long tokens) {
   const long long tiles = (hq / hk + 15) / 16;
   return grid_of((long long)batch * hk * tiles * ((tokens + UNIT - 1) / UNIT));
 }
-size_t prefix_bytes(int batch) { return ((size_t)(batch + 1) * 4 + 15) / 16 * 16; }
 int part_rows(int hq, int hk) { return hq / hk < 16 ? hq / hk : 16; }
 
 template <int D, bool FP8>
@@ -467,10 +503,12 @@ int launch(const Params& p, cudaStream_t stream) {
   }
   paged_attention_kernel<D, FP8><<<p.grid, THREADS, SMEM, stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return TW_ERR_LAUNCH;
+  if (p.grid == 1) return TW_OK;
   // the join's launch overlaps the end of the first kernel; it waits for it before it reads anything
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(p.batch * p.heads);
-  config.blockDim = dim3(128);
+  config.gridDim = dim3(p.grid - 1, p.rows);
+  config.blockDim = dim3(JOIN_THREADS);
+  config.dynamicSmemBytes = p.grid * sizeof(float);
   config.stream = stream;
   cudaLaunchAttribute early;
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -487,7 +525,7 @@ bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_
 
 extern "C" size_t tw_paged_attention_workspace(int batch, int hq, int hk, int dim, long long tokens) {
   if (batch <= 0 || hk <= 0 || hq <= 0 || hq % hk || dim <= 0 || tokens < 0) return 0;
-  return prefix_bytes(batch) + (size_t)grid_of(batch, hq, hk, tokens) * 2 * part_rows(hq, hk) * (dim + 2) * 4;
+  return (size_t)grid_of(batch, hq, hk, tokens) * (16 + 2 * part_rows(hq, hk) * (dim + 2) * 4);
 }
 
 extern "C" int tw_paged_attention(const TwPagedAttentionArgs* a, void* stream) {
@@ -518,8 +556,8 @@ extern "C" int tw_paged_attention(const TwPagedAttentionArgs* a, void* stream) {
   p.pages = a->pages; p.max_pages = a->max_pages; p.rows = part_rows(a->hq, a->hk); p.grid = grid_of(a->batch, a->hq, a->hk, tokens);
   while ((1 << p.page_shift) < a->page) ++p.page_shift;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-  p.prefix = reinterpret_cast<int*>(ws);
-  p.part_ml = reinterpret_cast<float*>(ws + prefix_bytes(a->batch));
+  p.starts = reinterpret_cast<int4*>(ws);
+  p.part_ml = reinterpret_cast<float*>(p.starts + p.grid);
   p.part_o = p.part_ml + (size_t)p.grid * 2 * p.rows * 2;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (a->dim == 128) return a->fp8 ? launch<128, true>(p, st) : launch<128, false>(p, st);
