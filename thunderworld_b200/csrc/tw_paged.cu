@@ -31,7 +31,8 @@ struct Params {
   const int *lengths, *slots;
   const float *k_scale, *v_scale;
   __nv_bfloat16* out; float* lse;
-  int4* starts;                     // [grid] batch entry, head, tile and number of tiles where a CTA's run begins; batch -1: no run
+  long long* all;                   // units in all
+  int4* starts;                     // [grid] batch entry, head, tile and number of tiles where a CTA's run begins
   float *part_o, *part_ml;          // [grid][2][rows][dim], [grid][2][rows][2]
   int* status;
   float scale_log2;
@@ -50,6 +51,9 @@ __device__ __forceinline__ int tokens_of(const Params& p, int b, int& slot) {
 }
 __device__ __forceinline__ int units_of(int tokens) { return (tokens + UNIT - 1) / UNIT; }
 
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
@@ -93,11 +97,12 @@ struct Cursor {
   int unit, b, h, tile, units, tokens, slot;       // tile: of the sequence's `units`
 };
 
-template <int D, bool FP8>
+// WIDE: more than 8 query rows per tile; else the lower half of the 16 rows is all there is, and nothing is computed for the rest.
+template <int D, bool FP8, bool WIDE>
 __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __grid_constant__ Params p) {
   constexpr int ROW = D * (FP8 ? 1 : 2), CHUNKS = ROW / 16, TILE = 16 * ROW;      // bytes of a row, of 16 rows
-  constexpr int STAGES = 2;
-  extern __shared__ __align__(128) uint8_t dynamic[];                             // [WARPS][STAGES][K, V][16 rows]
+  constexpr int STAGES = 2, HALVES = WIDE ? 2 : 1;
+  extern __shared__ __align__(128) uint8_t dynamic[];                             // [WARPS][STAGES][K, V][16 rows], from a multiple of 256
   __shared__ float gather[WARPS * JOIN_ROWS * D];
   __shared__ float part_m[WARPS][16], part_l[WARPS][16];
   __shared__ int sums[WARPS + 1], start_b, start_offset;
@@ -133,10 +138,8 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
     }
   }
   __syncthreads();
-  if (unit0 >= unit1) {
-    if (threadIdx.x == 0) p.starts[blockIdx.x] = make_int4(-1, 0, 0, 0);
-    return;
-  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.all = all;
+  if (unit0 >= unit1) return;
   const int count = (int)(unit1 - unit0);
 
   auto enter = [&](Cursor& c) { c.tokens = tokens_of(p, c.b, c.slot); c.units = units_of(c.tokens); };
@@ -157,54 +160,73 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
   };
 
   // ---- copies: 16 tokens' rows of K and of V to the warp's ring ---------------------------------------------
-  const uint32_t ring = tw::smem_u32(dynamic) + warp * STAGES * 2 * TILE;
+  // rows begin at multiples of 256, so that a chunk's place in its row can be had by exclusive or
+  const uint32_t ring = ((tw::smem_u32(dynamic) + 255) & ~255u) + warp * STAGES * 2 * TILE;
   constexpr int LANES = CHUNKS, STEP = 32 / LANES, COPIES = 16 / STEP;            // lanes per row, rows per instruction
+  constexpr int PLACES = STEP >= 8 ? 1 : 8 / STEP;                                // different swizzles of a lane's chunks
   const int copy_row = lane / LANES, copy_chunk = lane % LANES;
+  uint32_t place[PLACES];
+#pragma unroll
+  for (int i = 0; i < PLACES; ++i) place[i] = copy_row * ROW + swizzled<CHUNKS>(copy_chunk, i * STEP + copy_row) * 16;
   Cursor in;
   begin(in);
   if (threadIdx.x == 0) p.starts[blockIdx.x] = make_int4(in.b, in.h, in.tile, in.units);
-  uint32_t masks[STAGES];              // tokens of a stage that count
-  auto fetch = [&](int stage) {
+  const int in_page = (1 << p.page_shift) - 1;
+  int next_page = 0;                   // where the tokens lie that are fetched next: looked up a tile ahead
+  auto look_up = [&]() {
+    const int t0 = in.tile * UNIT + warp * 16;
+    if (p.page_shift >= 4 && t0 < in.tokens) next_page = __ldg(p.table + in.slot * p.table_stride + (t0 >> p.page_shift));
+  };
+  look_up();
+  // Starts the copies of the next tile; returns which of its tokens count.
+  auto fetch = [&](uint32_t to) -> uint32_t {
     uint32_t mask = 0;
     const int t0 = in.tile * UNIT + warp * 16;
     if (in.unit < count && t0 < in.tokens) {
       const int live = min(in.tokens - t0, 16), kv = in.h / p.tiles;
-      const int* entries = p.table + in.slot * p.table_stride;
-      const uint32_t to = ring + stage * 2 * TILE;
-      const long long k_at = kv * p.k_head, v_at = kv * p.v_head;
-      int page = -1;
-      if (p.page_shift >= 4) {         // the 16 tokens lie in one page
-        page = __ldg(entries + (t0 >> p.page_shift));
-        if (page < 0 || page >= p.pages) { if (lane == 0) report(p); } else mask = 0xffffu >> (16 - live);
-      }
+      if (p.page_shift >= 4) {         // the 16 tokens lie in one page, one behind the other
+        const bool inside = next_page >= 0 && next_page < p.pages;
+        if (!inside && lane == 0) report(p);
+        const long long page = inside ? next_page : 0, row = (long long)(t0 & in_page) * ROW + lane * 16;
+        const uint8_t *k = p.k + page * p.k_page + kv * p.k_head + row, *v = p.v + page * p.v_page + kv * p.v_head + row;
+        if (inside) mask = 0xffffu >> (16 - live);
+        if (mask == 0xffffu) {
 #pragma unroll
-      for (int i = 0; i < COPIES; ++i) {
-        const int r = i * STEP + copy_row, token = t0 + r;
-        bool valid = r < live;
-        if (p.page_shift < 4) {
-          page = valid ? __ldg(entries + (token >> p.page_shift)) : -1;
-          if (valid && (page < 0 || page >= p.pages)) { report(p); valid = false; }
+          for (int i = 0; i < COPIES; ++i) {
+            copy16(to + place[i % PLACES] + i * 512, k + i * 512);
+            copy16(to + TILE + place[i % PLACES] + i * 512, v + i * 512);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < COPIES; ++i) {
+            const bool valid = mask >> (i * STEP + copy_row) & 1u;
+            copy16(to + place[i % PLACES] + i * 512, valid ? k + i * 512 : p.k, valid ? 16 : 0);
+            copy16(to + TILE + place[i % PLACES] + i * 512, valid ? v + i * 512 : p.v, valid ? 16 : 0);
+          }
+        }
+      } else {
+        const int* entries = p.table + in.slot * p.table_stride;
+#pragma unroll
+        for (int i = 0; i < COPIES; ++i) {
+          const int r = i * STEP + copy_row, token = t0 + r;
+          bool valid = r < live;
+          const long long page = valid ? __ldg(entries + (token >> p.page_shift)) : 0;
+          if (page < 0 || page >= p.pages) { report(p); valid = false; }
           // one bit per row, from the first lane of each row
           const uint32_t votes = __ballot_sync(0xffffffffu, valid);
 #pragma unroll
           for (int j = 0; j < STEP; ++j) mask |= (votes >> (j * LANES) & 1u) << (i * STEP + j);
-        } else {
-          valid = valid && mask;
+          const long long row = (long long)(token & in_page) * ROW + copy_chunk * 16;
+          copy16(to + place[i % PLACES] + i * 512, valid ? p.k + page * p.k_page + kv * p.k_head + row : p.k, valid ? 16 : 0);
+          copy16(to + TILE + place[i % PLACES] + i * 512, valid ? p.v + page * p.v_page + kv * p.v_head + row : p.v, valid ? 16 : 0);
         }
-        const long long row = (long long)(token & ((1 << p.page_shift) - 1)) * ROW + copy_chunk * 16;
-        const uint32_t at = r * ROW + swizzled<CHUNKS>(copy_chunk, r) * 16;
-        const uint8_t* k = valid ? p.k + page * p.k_page + k_at + row : p.k;
-        const uint8_t* v = valid ? p.v + page * p.v_page + v_at + row : p.v;
-        copy16(to + at, k, valid ? 16 : 0);
-        copy16(to + TILE + at, v, valid ? 16 : 0);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    masks[stage] = mask;
-    if (in.unit < count) advance(in);
+    if (in.unit < count) { advance(in); if (in.unit < count) look_up(); }
+    return mask;
   };
-#pragma unroll
-  for (int s = 0; s < STAGES; ++s) fetch(s);
+  uint32_t stage = ring, mask = fetch(ring), next_mask = fetch(ring + 2 * TILE);
 
   // ---- products -----------------------------------------------------------------------------------------------------
   uint32_t q[D / 16][4];               // A fragments; with E4M3 pages lane t holds channels 4 t ... 4 t + 3 of each 16
@@ -214,10 +236,15 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
   bool first_segment = true;
   bool fresh = true;
   const bool begins_inside = at.tile != 0;
+  // Lane addresses of the fragment loads, of a tile at address 0; chunk 2 j of a row is 32 j further, by exclusive or.
+  // keys: tokens 0-7 and 8-15 (lane / 16) of channels 16 j ... + 7 and + 8 ... + 15 (lane / 8 % 2); values: tokens 0-7 and 8-15
+  // (lane / 8 % 2) of chunks 2 c and 2 c + 1 (lane / 16)
+  const int key_row = (lane & 7) + (lane >> 4) * 8, value_row = lane & 15;
+  const uint32_t key_lane = key_row * ROW + swizzled<CHUNKS>(lane >> 3 & 1, key_row) * 16;
+  const uint32_t value_lane = value_row * ROW + swizzled<CHUNKS>(lane >> 4, value_row) * 16;
+  const uint32_t fp8_lane = g * ROW + swizzled<CHUNKS>(0, g) * 16 + t * 4;       // row g + 8 has the same swizzle
   while (at.unit < count) {
-#pragma unroll
-    for (int stage = 0; stage < STAGES; ++stage) {
-      if (at.unit >= count) break;
+    {
       if (fresh) {
         fresh = false;
         const int kv = at.h / p.tiles, row0 = (at.h - kv * p.tiles) * 16;
@@ -236,7 +263,7 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
         score_scale[0] = score_scale[1] = p.scale_log2 * k_scale;
         if (FP8) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {                   // rows g and g + 8 to the range of f16, as the largest finite value says
+          for (int h = 0; h < HALVES; ++h) {              // rows g and g + 8 to the range of f16, as the largest finite value says
             unsigned top = 0;
 #pragma unroll
             for (int j = 0; j < D / 16; ++j)
@@ -267,7 +294,6 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
 
       asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
       __syncwarp();
-      const uint32_t mask = masks[stage], keys = ring + stage * 2 * TILE, values = keys + TILE;
       if (mask) {
         float s[2][4];
 #pragma unroll
@@ -278,14 +304,12 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
               uint32_t w;
-              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(keys + (n * 8 + g) * ROW + swizzled<CHUNKS>(j, n * 8 + g) * 16 + t * 4) : "memory");
+              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(((stage + fp8_lane) ^ (j * 16)) + n * 8 * ROW) : "memory");
               mma<true>(s[n], q[j], e4m3_to_f16(w & 0xffffu), e4m3_to_f16(w >> 16));
             }
           } else {
-            // matrices: tokens 0-7 and 8-15 (lane / 16) of channels 16 j ... + 7 and + 8 ... + 15 (lane / 8 % 2)
             uint32_t b[4];
-            const int r = (lane & 7) + (lane >> 4) * 8, c = j * 2 + (lane >> 3 & 1);
-            ldsm4(b, keys + r * ROW + swizzled<CHUNKS>(c, r) * 16);
+            ldsm4(b, (stage + key_lane) ^ (j * 32));
             mma<false>(s[0], q[j], b[0], b[1]);
             mma<false>(s[1], q[j], b[2], b[3]);
           }
@@ -295,50 +319,52 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            s[n][i] *= score_scale[i >> 1];
-            if (!(mask >> (n * 8 + t * 2 + (i & 1)) & 1u)) s[n][i] = -INFINITY;
-            top[i >> 1] = fmaxf(top[i >> 1], s[n][i]);
-          }
+          for (int i = 0; i < 2 * HALVES; ++i) s[n][i] *= score_scale[i >> 1];
+        if (mask != 0xffffu) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 2 * HALVES; ++i)
+              if (!(mask >> (n * 8 + t * 2 + (i & 1)) & 1u)) s[n][i] = -INFINITY;
+        }
+        bool higher = false;
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          top[h] = fmaxf(fmaxf(top[h], fmaxf(s[0][2 * h], s[0][2 * h + 1])), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
           top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
           top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+          higher = higher || top[h] > m[h];
         }
-        if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
-          const float a0 = weight_of(m[0], top[0]), a1 = weight_of(m[1], top[1]);
-          m[0] = top[0];
-          m[1] = top[1];
-          l[0] *= a0;
-          l[1] *= a1;
+        if (__any_sync(0xffffffffu, higher)) {
 #pragma unroll
-          for (int n = 0; n < D / 8; ++n) { o[n][0] *= a0; o[n][1] *= a0; o[n][2] *= a1; o[n][3] *= a1; }
-        }
-        const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+          for (int h = 0; h < HALVES; ++h) {
+            const float a = weight_of(m[h], top[h]);
+            m[h] = top[h];
+            l[h] *= a;
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            s[n][i] = exp2_fast(s[n][i] - ref[i >> 1]);
-            l[i >> 1] += s[n][i];
+            for (int n = 0; n < D / 8; ++n) { o[n][2 * h] *= a; o[n][2 * h + 1] *= a; }
           }
-        uint32_t hi[4], lo[4];         // probabilities as an A fragment: rows g, g + 8; tokens 2 t, 2 t + 8
+        }
+        uint32_t hi[4] = {}, lo[4] = {};                  // probabilities as an A fragment: rows g, g + 8; tokens 2 t, 2 t + 8
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float x = s[i >> 1][(i & 1) * 2], y = s[i >> 1][(i & 1) * 2 + 1];
-          if (FP8) {
-            hi[i] = pack_f16(x, y);
-          } else {
-            hi[i] = pack_bf16(x, y);
-            lo[i] = pack_bf16(x - tw::bf16_bits_to_float(hi[i] & 0xffffu), y - tw::bf16_bits_to_float(hi[i] >> 16));
+          const int h = i & 1;
+          if (h < HALVES) {
+            const float ref = m[h] == -INFINITY ? 0.f : m[h];
+            const float x = exp2_fast(s[i >> 1][h * 2] - ref), y = exp2_fast(s[i >> 1][h * 2 + 1] - ref);
+            l[h] += x + y;
+            if (FP8) {
+              hi[i] = pack_f16(x, y);
+            } else {
+              hi[i] = pack_bf16(x, y);
+              lo[i] = pack_bf16(x - tw::bf16_bits_to_float(hi[i] & 0xffffu), y - tw::bf16_bits_to_float(hi[i] >> 16));
+            }
           }
         }
 #pragma unroll
         for (int c = 0; c < CHUNKS / 2; ++c) {
-          // matrices: tokens 0-7 and 8-15 (lane / 8 % 2) of chunks 2 c and 2 c + 1 (lane / 16)
           uint32_t b[4];
-          const int r = lane & 15, ch = c * 2 + (lane >> 4);
-          ldsm4_trans(b, values + r * ROW + swizzled<CHUNKS>(ch, r) * 16);
+          ldsm4_trans(b, (stage + TILE + value_lane) ^ (c * 32));
           if (FP8) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {                 // a chunk's 16 channels: the even ones and the odd ones
@@ -355,7 +381,9 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
         }
       }
       __syncwarp();
-      fetch(stage);
+      mask = next_mask;
+      next_mask = fetch(stage);
+      stage = 2 * ring + 2 * TILE - stage;               // the other one
 
       const bool last = at.tile + 1 == at.units;
       if (last || at.unit + 1 == count) {
@@ -363,7 +391,7 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
         const bool whole = last && !(first_segment && begins_inside);
         const int kv = at.h / p.tiles, row0 = (at.h - kv * p.tiles) * 16, rows = min(p.group - row0, 16);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < HALVES; ++h) {
           l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
           l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
           if (t == 0) { part_m[warp][g + 8 * h] = m[h]; part_l[warp][g + 8 * h] = l[h]; }
@@ -371,7 +399,7 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
         const float v_scale = p.v_scale ? __ldg(p.v_scale + kv) : 1.f;
         for (int r0 = 0; r0 < rows; r0 += JOIN_ROWS) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < HALVES; ++h) {
             const int r = g + 8 * h - r0;
             if (r >= 0 && r < JOIN_ROWS) {
               float* to = gather + (warp * JOIN_ROWS + r) * D;
@@ -419,33 +447,39 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
 
 // Joins what several CTAs have of one (sequence, head tile): a block per border between two CTAs' runs and query row, which works
 // if its border is the first one inside the sequence.
-constexpr int JOIN_THREADS = 256;
+constexpr int JOIN_THREADS = 256;                          // CTAs of a run: 148 x 3 at most, under 2 JOIN_THREADS
 template <int D>
 __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const __grid_constant__ Params p) {
   extern __shared__ float weights[];                       // [grid]
   __shared__ float reduce[JOIN_THREADS / 32], sums[JOIN_THREADS / D][D];
   asm volatile("griddepcontrol.wait;" ::: "memory");       // the parts are written
   const int border = blockIdx.x + 1, r = blockIdx.y;
+  const long long all = *p.all, owners = min(all, (long long)p.grid);
+  if (border >= owners) return;
   const int4 here = p.starts[border], before = p.starts[border - 1];
-  if (here.x < 0 || here.z == 0) return;                   // no run, or one that begins with its sequence
+  if (here.z == 0) return;                                 // this run begins with its sequence
   const bool same = before.x == here.x && before.y == here.y;
   if (same && before.z > 0) return;                        // the run before begins inside the same sequence
   const int kv = here.y / p.tiles, row0 = (here.y - kv * p.tiles) * 16;
   if (row0 + r >= p.group) return;
-  // parts: the last of the run before (its first, if that begins with this sequence), and the first of every run that begins in it
-  __shared__ int after;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) after = p.grid;
-  __syncthreads();
-  for (int c = border + threadIdx.x; c < p.grid; c += JOIN_THREADS) {
-    const int4 x = p.starts[c];
-    if (x.x != here.x || x.y != here.y) { atomicMin(&after, c); break; }
-  }
-  __syncthreads();
-  const int parts = after - border + 1;
+  // CTA c has the units [all c / owners, all (c + 1) / owners): that of unit u is the last c with all c / owners <= u. The parts:
+  // the last of the run before (its first, if that begins with this sequence), and the first of every run that begins in it.
+  const long long end = all * border / owners - here.z + here.w;
+  const int parts = (int)((end * owners + all - 1) / all) - border + 1;
   auto slot_of = [&](int i) { return ((long long)(border - 1 + i) * 2 + (i == 0 && !same ? 1 : 0)) * p.rows + r; };
-  float top = -INFINITY;
-  for (int i = threadIdx.x; i < parts; i += JOIN_THREADS) { weights[i] = p.part_ml[slot_of(i) * 2]; top = fmaxf(top, weights[i]); }
+  float top = -INFINITY, sum = 0.f;
+  float mine[2] = {}, own_l[2] = {};                       // of the parts threadIdx.x and + JOIN_THREADS: there are fewer than 2 JOIN_THREADS
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = threadIdx.x + j * JOIN_THREADS;
+    if (i < parts) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot_of(i) * 2);
+      mine[j] = ml.x;
+      own_l[j] = ml.y;
+      top = fmaxf(top, ml.x);
+    }
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) reduce[warp] = top;
@@ -453,10 +487,10 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const __grid_c
 #pragma unroll
   for (int w = 0; w < JOIN_THREADS / 32; ++w) top = fmaxf(top, reduce[w]);
   __syncthreads();
-  float sum = 0.f;
-  for (int i = threadIdx.x; i < parts; i += JOIN_THREADS) {
-    weights[i] = weight_of(weights[i], top);
-    sum += weights[i] * p.part_ml[slot_of(i) * 2 + 1];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = threadIdx.x + j * JOIN_THREADS;
+    if (i < parts) { weights[i] = weight_of(mine[j], top); sum += weights[i] * own_l[j]; }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -488,20 +522,20 @@ int grid_of(int batch, int hq, int hk, long long tokens) {
 }
 int part_rows(int hq, int hk) { return hq / hk < 16 ? hq / hk : 16; }
 
-template <int D, bool FP8>
+template <int D, bool FP8, bool WIDE>
 int launch(const Params& p, cudaStream_t stream) {
-  constexpr int SMEM = WARPS * 2 * 2 * 16 * D * (FP8 ? 1 : 2);
+  constexpr int SMEM = WARPS * 2 * 2 * 16 * D * (FP8 ? 1 : 2) + 256;
   static std::atomic<bool> configured[64];            // the shared-memory opt-in is a per-device attribute of the function
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) { (void)cudaGetLastError(); return TW_ERR_LAUNCH; }
   if (device >= 64 || !configured[device].load(std::memory_order_relaxed)) {
-    if (cudaFuncSetAttribute(paged_attention_kernel<D, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) {
+    if (cudaFuncSetAttribute(paged_attention_kernel<D, FP8, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) {
       (void)cudaGetLastError();
       return TW_ERR_LAUNCH;
     }
     if (device < 64) configured[device].store(true, std::memory_order_relaxed);
   }
-  paged_attention_kernel<D, FP8><<<p.grid, THREADS, SMEM, stream>>>(p);
+  paged_attention_kernel<D, FP8, WIDE><<<p.grid, THREADS, SMEM, stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return TW_ERR_LAUNCH;
   if (p.grid == 1) return TW_OK;
   // the join's launch overlaps the end of the first kernel; it waits for it before it reads anything
@@ -525,7 +559,7 @@ bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_
 
 extern "C" size_t tw_paged_attention_workspace(int batch, int hq, int hk, int dim, long long tokens) {
   if (batch <= 0 || hk <= 0 || hq <= 0 || hq % hk || dim <= 0 || tokens < 0) return 0;
-  return (size_t)grid_of(batch, hq, hk, tokens) * (16 + 2 * part_rows(hq, hk) * (dim + 2) * 4);
+  return (size_t)grid_of(batch, hq, hk, tokens) * (16 + 2 * part_rows(hq, hk) * (dim + 2) * 4) + 16;
 }
 
 extern "C" int tw_paged_attention(const TwPagedAttentionArgs* a, void* stream) {
@@ -556,10 +590,15 @@ extern "C" int tw_paged_attention(const TwPagedAttentionArgs* a, void* stream) {
   p.pages = a->pages; p.max_pages = a->max_pages; p.rows = part_rows(a->hq, a->hk); p.grid = grid_of(a->batch, a->hq, a->hk, tokens);
   while ((1 << p.page_shift) < a->page) ++p.page_shift;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-  p.starts = reinterpret_cast<int4*>(ws);
+  p.all = reinterpret_cast<long long*>(ws);
+  p.starts = reinterpret_cast<int4*>(ws + 16);
   p.part_ml = reinterpret_cast<float*>(p.starts + p.grid);
   p.part_o = p.part_ml + (size_t)p.grid * 2 * p.rows * 2;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->dim == 128) return a->fp8 ? launch<128, true>(p, st) : launch<128, false>(p, st);
-  return a->fp8 ? launch<64, true>(p, st) : launch<64, false>(p, st);
+  if (p.rows <= 8) {
+    if (a->dim == 128) return a->fp8 ? launch<128, true, false>(p, st) : launch<128, false, false>(p, st);
+    return a->fp8 ? launch<64, true, false>(p, st) : launch<64, false, false>(p, st);
+  }
+  if (a->dim == 128) return a->fp8 ? launch<128, true, true>(p, st) : launch<128, false, true>(p, st);
+  return a->fp8 ? launch<64, true, true>(p, st) : launch<64, false, true>(p, st);
 }
