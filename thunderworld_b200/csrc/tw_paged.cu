@@ -178,6 +178,12 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
     if (p.page_shift >= 4 && t0 < in.tokens) next_page = __ldg(p.table + in.slot * p.table_stride + (t0 >> p.page_shift));
   };
   look_up();
+  // the queries of the sequence entered, to where they are had quickly when its turn comes: a line per lane
+  auto warm = [&]() {
+    const int kv = in.h / p.tiles, row = (in.h - kv * p.tiles) * 16 + (lane >> 1);
+    if (row < p.group && (D == 128 || !(lane & 1)))
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(p.q + in.b * p.q_batch + (long long)(kv * p.group + row) * p.q_head + (lane & 1) * 64));
+  };
   // Starts the copies of the next tile; returns which of its tokens count.
   auto fetch = [&](uint32_t to) -> uint32_t {
     uint32_t mask = 0;
@@ -223,7 +229,13 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    if (in.unit < count) { advance(in); if (in.unit < count) look_up(); }
+    if (in.unit < count) {
+      advance(in);
+      if (in.unit < count) {
+        look_up();
+        if (in.tile == 0) warm();
+      }
+    }
     return mask;
   };
   uint32_t stage = ring, mask = fetch(ring), next_mask = fetch(ring + 2 * TILE);
@@ -445,73 +457,66 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
   }
 }
 
-// Joins what several CTAs have of one (sequence, head tile): a block per border between two CTAs' runs and query row, which works
-// if its border is the first one inside the sequence.
-constexpr int JOIN_THREADS = 256;                          // CTAs of a run: 148 x 3 at most, under 2 JOIN_THREADS
+// Joins what several CTAs have of one (sequence, head tile): a block per border between two CTAs' runs and JOIN_ROWS query rows,
+// which works if its border is the first one inside the sequence. 128 threads have a row, D / 2 channels by pairs and every second
+// (D 64: fourth) part each.
+constexpr int JOIN_THREADS = JOIN_ROWS * 128;
 template <int D>
 __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const __grid_constant__ Params p) {
-  extern __shared__ float weights[];                       // [grid]
-  __shared__ float reduce[JOIN_THREADS / 32], sums[JOIN_THREADS / D][D];
+  extern __shared__ float weights[];                       // [JOIN_ROWS][grid] maxima, then weights
+  __shared__ float reduce[JOIN_THREADS / 32];
+  __shared__ float2 sums[JOIN_ROWS][128];
   asm volatile("griddepcontrol.wait;" ::: "memory");       // the parts are written
-  const int border = blockIdx.x + 1, r = blockIdx.y;
+  const int border = blockIdx.x + 1;
   const long long all = *p.all, owners = min(all, (long long)p.grid);
   if (border >= owners) return;
   const int4 here = p.starts[border], before = p.starts[border - 1];
   if (here.z == 0) return;                                 // this run begins with its sequence
   const bool same = before.x == here.x && before.y == here.y;
   if (same && before.z > 0) return;                        // the run before begins inside the same sequence
-  const int kv = here.y / p.tiles, row0 = (here.y - kv * p.tiles) * 16;
-  if (row0 + r >= p.group) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kv = here.y / p.tiles, row0 = (here.y - kv * p.tiles) * 16, own = threadIdx.x >> 7, r = blockIdx.y * JOIN_ROWS + own;
+  const bool live = row0 + r < p.group && r < 16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = threadIdx.x & 127;
   // CTA c has the units [all c / owners, all (c + 1) / owners): that of unit u is the last c with all c / owners <= u. The parts:
   // the last of the run before (its first, if that begins with this sequence), and the first of every run that begins in it.
   const long long end = all * border / owners - here.z + here.w;
-  const int parts = (int)((end * owners + all - 1) / all) - border + 1;
+  const int parts = live ? (int)((end * owners + all - 1) / all) - border + 1 : 0;
   auto slot_of = [&](int i) { return ((long long)(border - 1 + i) * 2 + (i == 0 && !same ? 1 : 0)) * p.rows + r; };
+  float* w = weights + own * p.grid;
   float top = -INFINITY, sum = 0.f;
-  float mine[2] = {}, own_l[2] = {};                       // of the parts threadIdx.x and + JOIN_THREADS: there are fewer than 2 JOIN_THREADS
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int i = threadIdx.x + j * JOIN_THREADS;
-    if (i < parts) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot_of(i) * 2);
-      mine[j] = ml.x;
-      own_l[j] = ml.y;
-      top = fmaxf(top, ml.x);
-    }
-  }
+  for (int i = t; i < parts; i += 128) { w[i] = p.part_ml[slot_of(i) * 2]; top = fmaxf(top, w[i]); }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) reduce[warp] = top;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < JOIN_THREADS / 32; ++w) top = fmaxf(top, reduce[w]);
+  top = fmaxf(fmaxf(reduce[own * 4], reduce[own * 4 + 1]), fmaxf(reduce[own * 4 + 2], reduce[own * 4 + 3]));
   __syncthreads();
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int i = threadIdx.x + j * JOIN_THREADS;
-    if (i < parts) { weights[i] = weight_of(mine[j], top); sum += weights[i] * own_l[j]; }
+  for (int i = t; i < parts; i += 128) {                   // a thread's own
+    w[i] = weight_of(w[i], top);
+    sum += w[i] * p.part_ml[slot_of(i) * 2 + 1];
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) reduce[warp] = sum;
   __syncthreads();
-  sum = 0.f;
-#pragma unroll
-  for (int w = 0; w < JOIN_THREADS / 32; ++w) sum += reduce[w];
-  const int d = threadIdx.x % D, share = threadIdx.x / D;
-  float y = 0.f;
+  sum = reduce[own * 4] + reduce[own * 4 + 1] + reduce[own * 4 + 2] + reduce[own * 4 + 3];
+  const int pair = t % (D / 2), share = t / (D / 2);
+  float2 y = make_float2(0.f, 0.f);
 #pragma unroll 8
-  for (int i = share; i < parts; i += JOIN_THREADS / D) y += weights[i] * p.part_o[slot_of(i) * D + d];
-  sums[share][d] = y;
+  for (int i = share; i < parts; i += 256 / D) {
+    const float2 o = *reinterpret_cast<const float2*>(p.part_o + slot_of(i) * D + pair * 2);
+    y.x += w[i] * o.x;
+    y.y += w[i] * o.y;
+  }
+  sums[own][t] = y;
   __syncthreads();
-  if (share) return;
+  if (share || !live) return;
 #pragma unroll
-  for (int w = 1; w < JOIN_THREADS / D; ++w) y += sums[w][d];
+  for (int q = 1; q < 256 / D; ++q) { y.x += sums[own][q * (D / 2) + pair].x; y.y += sums[own][q * (D / 2) + pair].y; }
   const long long head = (long long)here.x * p.hk * p.group + kv * p.group + row0 + r;
-  const float v_scale = p.v_scale ? __ldg(p.v_scale + kv) : 1.f;
-  p.out[head * D + d] = __float2bfloat16_rn(sum == 0.f ? 0.f : y * v_scale / sum);
-  if (p.lse && d == 0) p.lse[head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945f;
+  const float scale = sum == 0.f ? 0.f : (p.v_scale ? __ldg(p.v_scale + kv) : 1.f) / sum;
+  *reinterpret_cast<uint32_t*>(p.out + head * D + pair * 2) = sum == 0.f ? 0u : pack_bf16(y.x * scale, y.y * scale);
+  if (p.lse && pair == 0) p.lse[head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945f;
 }
 
 // CTAs that run beside each other, for units of which there are at most `most`.
@@ -540,9 +545,9 @@ int launch(const Params& p, cudaStream_t stream) {
   if (p.grid == 1) return TW_OK;
   // the join's launch overlaps the end of the first kernel; it waits for it before it reads anything
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(p.grid - 1, p.rows);
+  config.gridDim = dim3(p.grid - 1, (p.rows + JOIN_ROWS - 1) / JOIN_ROWS);
   config.blockDim = dim3(JOIN_THREADS);
-  config.dynamicSmemBytes = p.grid * sizeof(float);
+  config.dynamicSmemBytes = p.grid * JOIN_ROWS * sizeof(float);
   config.stream = stream;
   cudaLaunchAttribute early;
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -575,7 +580,7 @@ extern "C" int tw_paged_attention(const TwPagedAttentionArgs* a, void* stream) {
   const int bytes = a->fp8 ? 1 : 2;
   if (misaligned(a->q, 4) || (a->q_stride_batch | a->q_stride_head) & 1 || misaligned(a->k_pages, 16) || misaligned(a->v_pages, 16) ||
       ((a->k_stride_page | a->k_stride_head | a->v_stride_page | a->v_stride_head) * bytes) % 16 || misaligned(a->workspace, 16) ||
-      misaligned(a->out, 2) || misaligned(a->table, 4) || misaligned(a->lengths, 4))
+      misaligned(a->out, 4) || misaligned(a->table, 4) || misaligned(a->lengths, 4))
     return TW_ERR_ALIGNMENT;
   Params p = {};
   p.q = static_cast<const __nv_bfloat16*>(a->q); p.q_batch = a->q_stride_batch; p.q_head = a->q_stride_head;
