@@ -4,7 +4,7 @@
 //
 // What bounds it is the read of the keys and values, once. The work is cut into units of 64 tokens of one (sequence, key head), in
 // that order, and the units are shared evenly by the CTAs that run beside each other, whatever the lengths (which only the device
-// knows): a CTA's run may begin and end inside a sequence, and what it has of such a one goes to the workspace, unnormalised, with
+// knows; putting the warps' parts of a sequence together costs about a unit and is counted as one): a CTA's run may begin and end inside a sequence, and what it has of such a one goes to the workspace, unnormalised, with
 // its maximum and sum; a second small launch joins these in their order. A call needs no zeroed state and no counter, so calls
 // on several streams, and captured ones, do not meet.
 // A warp takes 16 of a unit's tokens: it copies their rows (two units ahead) to a ring of its own, multiplies q (the group's heads,
@@ -31,7 +31,7 @@ struct Params {
   const int *lengths, *slots;
   const float *k_scale, *v_scale;
   __nv_bfloat16* out; float* lse;
-  long long* all;                   // units in all
+  int* all;                         // steps in all
   int4* starts;                     // [grid] batch entry, head, tile and number of tiles where a CTA's run begins
   float *part_o, *part_ml;          // [grid][2][rows][dim], [grid][2][rows][2]
   int* status;
@@ -92,9 +92,20 @@ __device__ __forceinline__ float weight_of(float m, float top) { return m == -IN
 // Place of 16-byte chunk c of row r in a tile of rows of CHUNKS chunks: what eight lanes read at once lies in different banks.
 template <int CHUNKS> __device__ __forceinline__ int swizzled(int c, int r) { return CHUNKS == 4 ? c ^ (r >> 1 & 3) : c ^ (r & 7); }
 
-// Where a CTA is in its run of units.
+// Shares of `all` steps: the first all % owners owners have a step more than the others.
+struct Shares {
+  int all, owners, per, more;
+  __device__ __forceinline__ Shares(int all_, int grid) : all(all_), owners(min(all_, grid)) { per = owners ? all / owners : 0; more = all - per * owners; }
+  __device__ __forceinline__ int begin(int c) const { return c * per + min(c, more); }
+  __device__ __forceinline__ int owner(int u) const { return u < more * (per + 1) ? u / (per + 1) : more + (u - more * (per + 1)) / per; }
+};
+// Where a warp is in its CTA's run: one cursor fetches, one multiplies. A sequence's steps are its units and, last, the joining of
+// its parts. What changes with the sequence only is kept in shared memory (every lane writes the same): registers are what
+// the kernel has least of.
+struct Sequence { int b, h, kv, slot, tokens; };
 struct Cursor {
-  int unit, b, h, tile, units, tokens, slot;       // tile: of the sequence's `units`
+  int left, tile, units;                           // steps left of the run; tile of the sequence's units
+  Sequence* of;
 };
 
 // WIDE: more than 8 query rows per tile; else the lower half of the 16 rows is all there is, and nothing is computed for the rest.
@@ -105,13 +116,14 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
   extern __shared__ __align__(128) uint8_t dynamic[];                             // [WARPS][STAGES][K, V][16 rows], from a multiple of 256
   __shared__ float gather[WARPS * JOIN_ROWS * D];
   __shared__ float part_m[WARPS][16], part_l[WARPS][16];
+  __shared__ float2 joined[16];
   __shared__ int sums[WARPS + 1], start_b, start_offset;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
   // ---- this CTA's run: the lengths' prefix sums, in units -----------------------------------------------------------
   const int per = (p.batch + THREADS - 1) / THREADS, first_b = min(threadIdx.x * per, p.batch), last_b = min(first_b + per, p.batch);
   int mine = 0, slot_unused;
-  for (int b = first_b; b < last_b; ++b) mine += units_of(tokens_of(p, b, slot_unused));
+  for (int b = first_b; b < last_b; ++b) { const int n = units_of(tokens_of(p, b, slot_unused)); mine += n ? n + 1 : 0; }
   int before = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) { const int x = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += x; }
@@ -120,44 +132,48 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
   int total = 0;
 #pragma unroll
   for (int w = 0; w < WARPS; ++w) { if (w == warp) before += total - mine; total += sums[w]; }
-  const long long all = (long long)total * p.heads, owners = min(all, (long long)p.grid);     // every owner has a unit at least
-  const long long unit0 = blockIdx.x < owners ? all * blockIdx.x / owners : 0, unit1 = blockIdx.x < owners ? all * (blockIdx.x + 1) / owners : 0;
-  {
-    int at = before;
-    for (int b = first_b; b < last_b; ++b) {
-      const int n = units_of(tokens_of(p, b, slot_unused));
-      if ((long long)at * p.heads <= unit0 && unit0 < (long long)(at + n) * p.heads) { start_b = b; start_offset = (int)(unit0 - (long long)at * p.heads); }
-      at += n;
-    }
-    // rows of empty sequences, dealt out over the CTAs
-    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-      if (tokens_of(p, b, slot_unused)) continue;
-      const long long head0 = (long long)b * p.hk * p.group, heads = p.hk * p.group;
-      for (long long e = threadIdx.x; e < heads * D; e += THREADS) p.out[head0 * D + e] = __float2bfloat16_rn(0.f);
-      if (p.lse) for (int e = threadIdx.x; e < heads; e += THREADS) p.lse[head0 + e] = -INFINITY;
-    }
+  const Shares shares(total * p.heads, p.grid);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.all = shares.all;
+  // rows of empty sequences, dealt out over the CTAs
+  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+    if (tokens_of(p, b, slot_unused)) continue;
+    const long long head0 = (long long)b * p.hk * p.group, heads = p.hk * p.group;
+    for (long long e = threadIdx.x; e < heads * D; e += THREADS) p.out[head0 * D + e] = __float2bfloat16_rn(0.f);
+    if (p.lse) for (int e = threadIdx.x; e < heads; e += THREADS) p.lse[head0 + e] = -INFINITY;
+  }
+  if ((int)blockIdx.x >= shares.owners) return;
+  const int step0 = shares.begin(blockIdx.x);
+  for (int b = first_b, at = before * p.heads; b < last_b; ++b) {
+    const int n = units_of(tokens_of(p, b, slot_unused)), steps = n ? (n + 1) * p.heads : 0;
+    if (at <= step0 && step0 < at + steps) { start_b = b; start_offset = step0 - at; }
+    at += steps;
   }
   __syncthreads();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *p.all = all;
-  if (unit0 >= unit1) return;
-  const int count = (int)(unit1 - unit0);
 
-  auto enter = [&](Cursor& c) { c.tokens = tokens_of(p, c.b, c.slot); c.units = units_of(c.tokens); };
-  auto begin = [&](Cursor& c) {
-    c.unit = 0;
-    c.b = start_b;
-    enter(c);
-    c.h = start_offset / c.units;
-    c.tile = start_offset - c.h * c.units;
+  __shared__ Sequence sequences[2][WARPS];
+  auto enter = [&](Cursor& c, int b) {
+    int slot;
+    const int tokens = tokens_of(p, b, slot);
+    c.of->b = b;
+    c.of->slot = slot;
+    c.of->tokens = tokens;
+    c.units = units_of(tokens);
   };
-  auto advance = [&](Cursor& c) {
-    ++c.unit;
-    if (++c.tile < c.units || c.unit >= count) return;
+  // to the next sequence, if the cursor is behind the units of its own
+  auto settle = [&](Cursor& c) {
+    if (c.tile < c.units) return;
+    --c.left;                                      // the joining step
     c.tile = 0;
-    if (++c.h < p.heads) return;
-    c.h = 0;
-    do { ++c.b; enter(c); } while (c.units == 0);
+    int b = c.of->b, h = c.of->h + 1;
+    __syncwarp();                                  // every lane has read what every lane writes now
+    if (h == p.heads) {
+      h = 0;
+      if (c.left > 0) do enter(c, ++b); while (c.units == 0);
+    }
+    c.of->h = h;
+    c.of->kv = h / p.tiles;
   };
+  auto advance = [&](Cursor& c) { --c.left; ++c.tile; settle(c); };
 
   // ---- copies: 16 tokens' rows of K and of V to the warp's ring ---------------------------------------------
   // rows begin at multiples of 256, so that a chunk's place in its row can be had by exclusive or
@@ -169,27 +185,37 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
 #pragma unroll
   for (int i = 0; i < PLACES; ++i) place[i] = copy_row * ROW + swizzled<CHUNKS>(copy_chunk, i * STEP + copy_row) * 16;
   Cursor in;
-  begin(in);
-  if (threadIdx.x == 0) p.starts[blockIdx.x] = make_int4(in.b, in.h, in.tile, in.units);
+  in.left = shares.begin(blockIdx.x + 1) - step0;
+  in.of = &sequences[0][warp];
+  enter(in, start_b);
+  const int start_h = start_offset / (in.units + 1);
+  in.of->h = start_h;
+  in.of->kv = start_h / p.tiles;
+  in.tile = start_offset - start_h * (in.units + 1);
+  settle(in);                          // a run that begins with a joining step leaves it to the owner of the sequence's last unit
+  Cursor at = in;
+  at.of = &sequences[1][warp];
+  *at.of = *in.of;
+  if (threadIdx.x == 0) p.starts[blockIdx.x] = make_int4(in.of->b, in.of->h, in.tile, in.units);
   const int in_page = (1 << p.page_shift) - 1;
   int next_page = 0;                   // where the tokens lie that are fetched next: looked up a tile ahead
   auto look_up = [&]() {
     const int t0 = in.tile * UNIT + warp * 16;
-    if (p.page_shift >= 4 && t0 < in.tokens) next_page = __ldg(p.table + in.slot * p.table_stride + (t0 >> p.page_shift));
+    if (p.page_shift >= 4 && t0 < in.of->tokens) next_page = __ldg(p.table + in.of->slot * p.table_stride + (t0 >> p.page_shift));
   };
   look_up();
   // the queries of the sequence entered, to where they are had quickly when its turn comes: a line per lane
   auto warm = [&]() {
-    const int kv = in.h / p.tiles, row = (in.h - kv * p.tiles) * 16 + (lane >> 1);
+    const int kv = in.of->kv, row = (in.of->h - kv * p.tiles) * 16 + (lane >> 1);
     if (row < p.group && (D == 128 || !(lane & 1)))
-      asm volatile("prefetch.global.L1 [%0];" ::"l"(p.q + in.b * p.q_batch + (long long)(kv * p.group + row) * p.q_head + (lane & 1) * 64));
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(p.q + in.of->b * p.q_batch + (long long)(kv * p.group + row) * p.q_head + (lane & 1) * 64));
   };
   // Starts the copies of the next tile; returns which of its tokens count.
   auto fetch = [&](uint32_t to) -> uint32_t {
     uint32_t mask = 0;
     const int t0 = in.tile * UNIT + warp * 16;
-    if (in.unit < count && t0 < in.tokens) {
-      const int live = min(in.tokens - t0, 16), kv = in.h / p.tiles;
+    if (in.left > 0 && t0 < in.of->tokens) {
+      const int live = min(in.of->tokens - t0, 16), kv = in.of->kv;
       if (p.page_shift >= 4) {         // the 16 tokens lie in one page, one behind the other
         const bool inside = next_page >= 0 && next_page < p.pages;
         if (!inside && lane == 0) report(p);
@@ -211,7 +237,7 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
           }
         }
       } else {
-        const int* entries = p.table + in.slot * p.table_stride;
+        const int* entries = p.table + in.of->slot * p.table_stride;
 #pragma unroll
         for (int i = 0; i < COPIES; ++i) {
           const int r = i * STEP + copy_row, token = t0 + r;
@@ -229,24 +255,22 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    if (in.unit < count) {
+    if (in.left > 0) {
       advance(in);
-      if (in.unit < count) {
+      if (in.left > 0) {
         look_up();
         if (in.tile == 0) warm();
       }
     }
     return mask;
   };
+  if (in.left > 0) warm();
   uint32_t stage = ring, mask = fetch(ring), next_mask = fetch(ring + 2 * TILE);
 
   // ---- products -----------------------------------------------------------------------------------------------------
   uint32_t q[D / 16][4];               // A fragments; with E4M3 pages lane t holds channels 4 t ... 4 t + 3 of each 16
   float o[D / 8][4], m[2], l[2], score_scale[2];
-  Cursor at;
-  begin(at);
-  bool first_segment = true;
-  bool fresh = true;
+  bool first_segment = true, fresh = true;
   const bool begins_inside = at.tile != 0;
   // Lane addresses of the fragment loads, of a tile at address 0; chunk 2 j of a row is 32 j further, by exclusive or.
   // keys: tokens 0-7 and 8-15 (lane / 16) of channels 16 j ... + 7 and + 8 ... + 15 (lane / 8 % 2); values: tokens 0-7 and 8-15
@@ -255,12 +279,11 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
   const uint32_t key_lane = key_row * ROW + swizzled<CHUNKS>(lane >> 3 & 1, key_row) * 16;
   const uint32_t value_lane = value_row * ROW + swizzled<CHUNKS>(lane >> 4, value_row) * 16;
   const uint32_t fp8_lane = g * ROW + swizzled<CHUNKS>(0, g) * 16 + t * 4;       // row g + 8 has the same swizzle
-  while (at.unit < count) {
-    {
+  while (at.left > 0) {
       if (fresh) {
         fresh = false;
-        const int kv = at.h / p.tiles, row0 = (at.h - kv * p.tiles) * 16;
-        const __nv_bfloat16* base = p.q + at.b * p.q_batch + (long long)(kv * p.group + row0) * p.q_head;
+        const int kv = at.of->kv, row0 = (at.of->h - kv * p.tiles) * 16;
+        const __nv_bfloat16* base = p.q + at.of->b * p.q_batch + (long long)(kv * p.group + row0) * p.q_head;
         const bool low = row0 + g < p.group, high = row0 + g + 8 < p.group;
         const __nv_bfloat16 *r0 = base + g * p.q_head, *r1 = base + (g + 8) * p.q_head;
 #pragma unroll
@@ -398,15 +421,29 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
       stage = 2 * ring + 2 * TILE - stage;               // the other one
 
       const bool last = at.tile + 1 == at.units;
-      if (last || at.unit + 1 == count) {
+      if (last || at.left == 1) {
         // ---- the sequence's, or the run's, end: the warps' parts together -------------------------------------------
         const bool whole = last && !(first_segment && begins_inside);
-        const int kv = at.h / p.tiles, row0 = (at.h - kv * p.tiles) * 16, rows = min(p.group - row0, 16);
+        const int kv = at.of->kv, row0 = (at.of->h - kv * p.tiles) * 16, rows = min(p.group - row0, 16);
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
           l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
           l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
           if (t == 0) { part_m[warp][g + 8 * h] = m[h]; part_l[warp][g + 8 * h] = l[h]; }
+        }
+        __syncthreads();
+        float own[HALVES];                                // weight of this warp's part
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          const int r = g + 8 * h;
+          const float top = fmaxf(fmaxf(part_m[0][r], part_m[1][r]), fmaxf(part_m[2][r], part_m[3][r]));
+          own[h] = weight_of(m[h], top);
+          if (warp == 0 && t == 0) {
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) sum += weight_of(part_m[w][r], top) * part_l[w][r];
+            joined[r] = make_float2(top, sum);
+          }
         }
         const float v_scale = p.v_scale ? __ldg(p.v_scale + kv) : 1.f;
         for (int r0 = 0; r0 < rows; r0 += JOIN_ROWS) {
@@ -419,32 +456,27 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
               for (int n = 0; n < D / 8; ++n) {
                 // E4M3: tiles 2 c and 2 c + 1 hold the even and odd channels of chunk c
                 const int d0 = FP8 ? (n >> 1) * 16 + t * 4 + (n & 1) : n * 8 + t * 2, d1 = d0 + (FP8 ? 2 : 1);
-                to[d0] = o[n][2 * h];
-                to[d1] = o[n][2 * h + 1];
+                to[d0] = o[n][2 * h] * own[h];
+                to[d1] = o[n][2 * h + 1] * own[h];
               }
             }
           }
           __syncthreads();
-          for (int e = threadIdx.x; e < JOIN_ROWS * D; e += THREADS) {
+#pragma unroll 1
+          for (int e = threadIdx.x; e < min(rows - r0, JOIN_ROWS) * D; e += THREADS) {
             const int r = r0 + e / D, d = e % D;
-            if (r >= rows) break;
-            float top = part_m[0][r], sum = 0.f, y = 0.f;
+            const float2 ml = joined[r];
+            float y = 0.f;
 #pragma unroll
-            for (int w = 1; w < WARPS; ++w) top = fmaxf(top, part_m[w][r]);
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) {
-              const float a = weight_of(part_m[w][r], top);
-              sum += a * part_l[w][r];
-              y += a * gather[(w * JOIN_ROWS + r - r0) * D + d];
-            }
+            for (int w = 0; w < WARPS; ++w) y += gather[w * JOIN_ROWS * D + e];
             if (whole) {
-              const long long head = (long long)at.b * p.hk * p.group + kv * p.group + row0 + r;
-              p.out[head * D + d] = __float2bfloat16_rn(sum == 0.f ? 0.f : y * v_scale / sum);
-              if (p.lse && d == 0) p.lse[head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945f;
+              const long long head = (long long)at.of->b * p.hk * p.group + kv * p.group + row0 + r;
+              p.out[head * D + d] = __float2bfloat16_rn(ml.y == 0.f ? 0.f : y * v_scale / ml.y);
+              if (p.lse && d == 0) p.lse[head] = ml.y == 0.f ? -INFINITY : (ml.x + log2f(ml.y)) * 0.693147180559945f;
             } else {
               const long long slot = ((long long)blockIdx.x * 2 + (first_segment ? 0 : 1)) * p.rows + r;
               p.part_o[slot * D + d] = y;
-              if (d == 0) { p.part_ml[slot * 2] = top; p.part_ml[slot * 2 + 1] = sum; }
+              if (d == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = ml;
             }
           }
           __syncthreads();
@@ -453,7 +485,6 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
         fresh = true;
       }
       advance(at);
-    }
   }
 }
 
@@ -468,8 +499,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const __grid_c
   __shared__ float2 sums[JOIN_ROWS][128];
   asm volatile("griddepcontrol.wait;" ::: "memory");       // the parts are written
   const int border = blockIdx.x + 1;
-  const long long all = *p.all, owners = min(all, (long long)p.grid);
-  if (border >= owners) return;
+  const Shares shares(*p.all, p.grid);
+  if (border >= shares.owners) return;
   const int4 here = p.starts[border], before = p.starts[border - 1];
   if (here.z == 0) return;                                 // this run begins with its sequence
   const bool same = before.x == here.x && before.y == here.y;
@@ -477,10 +508,9 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const __grid_c
   const int kv = here.y / p.tiles, row0 = (here.y - kv * p.tiles) * 16, own = threadIdx.x >> 7, r = blockIdx.y * JOIN_ROWS + own;
   const bool live = row0 + r < p.group && r < 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = threadIdx.x & 127;
-  // CTA c has the units [all c / owners, all (c + 1) / owners): that of unit u is the last c with all c / owners <= u. The parts:
-  // the last of the run before (its first, if that begins with this sequence), and the first of every run that begins in it.
-  const long long end = all * border / owners - here.z + here.w;
-  const int parts = live ? (int)((end * owners + all - 1) / all) - border + 1 : 0;
+  // the parts: the last of the run before (its first, if that begins with this sequence), and the first of every run that begins
+  // in it, up to the owner of its last unit
+  const int parts = live ? shares.owner(shares.begin(border) - here.z + here.w - 1) - border + 2 : 0;
   auto slot_of = [&](int i) { return ((long long)(border - 1 + i) * 2 + (i == 0 && !same ? 1 : 0)) * p.rows + r; };
   float* w = weights + own * p.grid;
   float top = -INFINITY, sum = 0.f;
@@ -523,7 +553,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const __grid_c
 int grid_of(long long most) { const long long fit = 148 * 3; return (int)(most < 1 ? 1 : most < fit ? most : fit); }
 int grid_of(int batch, int hq, int hk, long long tokens) {
   const long long tiles = (hq / hk + 15) / 16;
-  return grid_of((long long)batch * hk * tiles * ((tokens + UNIT - 1) / UNIT));
+  return grid_of((long long)batch * hk * tiles * ((tokens + UNIT - 1) / UNIT + 1));
 }
 int part_rows(int hq, int hk) { return hq / hk < 16 ? hq / hk : 16; }
 
@@ -575,7 +605,7 @@ extern "C" int tw_paged_attention(const TwPagedAttentionArgs* a, void* stream) {
   const long long tokens = (long long)a->max_pages * a->page;
   const int tiles = (a->hq / a->hk + 15) / 16, heads = a->hk * tiles;
   if (a->page > (1 << 20) || tokens > (1LL << 30) || (long long)a->batch * heads > (1 << 30) ||
-      (long long)a->batch * ((tokens + UNIT - 1) / UNIT) > (1LL << 31) - 1)
+      (long long)a->batch * heads * ((tokens + UNIT - 1) / UNIT + 1) > (1LL << 31) - 1)
     return TW_ERR_TOO_LARGE;
   const int bytes = a->fp8 ? 1 : 2;
   if (misaligned(a->q, 4) || (a->q_stride_batch | a->q_stride_head) & 1 || misaligned(a->k_pages, 16) || misaligned(a->v_pages, 16) ||
@@ -595,7 +625,7 @@ extern "C" int tw_paged_attention(const TwPagedAttentionArgs* a, void* stream) {
   p.pages = a->pages; p.max_pages = a->max_pages; p.rows = part_rows(a->hq, a->hk); p.grid = grid_of(a->batch, a->hq, a->hk, tokens);
   while ((1 << p.page_shift) < a->page) ++p.page_shift;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-  p.all = reinterpret_cast<long long*>(ws);
+  p.all = reinterpret_cast<int*>(ws);
   p.starts = reinterpret_cast<int4*>(ws + 16);
   p.part_ml = reinterpret_cast<float*>(p.starts + p.grid);
   p.part_o = p.part_ml + (size_t)p.grid * 2 * p.rows * 2;
