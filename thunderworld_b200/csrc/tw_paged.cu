@@ -31,8 +31,7 @@ struct Params {
   const int *lengths, *slots;
   const float *k_scale, *v_scale;
   __nv_bfloat16* out; float* lse;
-  int* all;                         // steps in all
-  int4* starts;                     // [grid] batch entry, head, tile and number of tiles where a CTA's run begins
+  int4* borders;                    // [grid] what to join where a CTA's run begins: number of parts (0: nothing), first part, head, rows
   float *part_o, *part_ml;          // [grid][2][rows][dim], [grid][2][rows][2]
   int* status;
   float scale_log2;
@@ -133,7 +132,6 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
 #pragma unroll
   for (int w = 0; w < WARPS; ++w) { if (w == warp) before += total - mine; total += sums[w]; }
   const Shares shares(total * p.heads, p.grid);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *p.all = shares.all;
   // rows of empty sequences, dealt out over the CTAs
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
     if (tokens_of(p, b, slot_unused)) continue;
@@ -141,7 +139,10 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
     for (long long e = threadIdx.x; e < heads * D; e += THREADS) p.out[head0 * D + e] = __float2bfloat16_rn(0.f);
     if (p.lse) for (int e = threadIdx.x; e < heads; e += THREADS) p.lse[head0 + e] = -INFINITY;
   }
-  if ((int)blockIdx.x >= shares.owners) return;
+  if ((int)blockIdx.x >= shares.owners) {
+    if (threadIdx.x == 0) p.borders[blockIdx.x] = make_int4(0, 0, 0, 0);
+    return;
+  }
   const int step0 = shares.begin(blockIdx.x);
   for (int b = first_b, at = before * p.heads; b < last_b; ++b) {
     const int n = units_of(tokens_of(p, b, slot_unused)), steps = n ? (n + 1) * p.heads : 0;
@@ -196,7 +197,18 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
   Cursor at = in;
   at.of = &sequences[1][warp];
   *at.of = *in.of;
-  if (threadIdx.x == 0) p.starts[blockIdx.x] = make_int4(in.of->b, in.of->h, in.tile, in.units);
+  if (threadIdx.x == 0) {
+    // A run that begins inside a sequence, the first one to: the parts are the last of the run before (its first, if that begins
+    // with the sequence, or with the joining step before it), and the first of every run from this one to the owner of the sequence's last unit.
+    int4 border = make_int4(0, 0, 0, 0);
+    if (in.left > 0 && in.tile > 0) {
+      const int begin = step0 - in.tile, previous = shares.begin((int)blockIdx.x - 1), row0 = (in.of->h - in.of->kv * p.tiles) * 16;
+      if (previous <= begin)
+        border = make_int4(shares.owner(begin + in.units - 1) - (int)blockIdx.x + 2, ((int)blockIdx.x - 1) * 2 + (previous < begin - 1 ? 1 : 0),
+                           (in.of->b * p.hk + in.of->kv) * p.group + row0, min(p.group - row0, 16));
+    }
+    p.borders[blockIdx.x] = border;
+  }
   const int in_page = (1 << p.page_shift) - 1;
   int next_page = 0;                   // where the tokens lie that are fetched next: looked up a tile ahead
   auto look_up = [&]() {
@@ -488,65 +500,57 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
   }
 }
 
-// Joins what several CTAs have of one (sequence, head tile): a block per border between two CTAs' runs and JOIN_ROWS query rows,
-// which works if its border is the first one inside the sequence. 128 threads have a row, D / 2 channels by pairs and every second
-// (D 64: fourth) part each.
-constexpr int JOIN_THREADS = JOIN_ROWS * 128;
+// Joins what several CTAs have of one (sequence, head tile): a block per border between two runs and JOIN_ROWS query rows. Four
+// warps have a row, each every fourth part.
+constexpr int JOIN_WARPS = 4, JOIN_THREADS = JOIN_ROWS * JOIN_WARPS * 32;
 template <int D>
 __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const __grid_constant__ Params p) {
-  extern __shared__ float weights[];                       // [JOIN_ROWS][grid] maxima, then weights
-  __shared__ float reduce[JOIN_THREADS / 32];
-  __shared__ float2 sums[JOIN_ROWS][128];
+  constexpr int VEC = D / 32;                              // channels of a lane
+  struct __align__(VEC * 4) Channels { float v[VEC]; };
+  __shared__ Channels sums[JOIN_ROWS][JOIN_WARPS][32];
   asm volatile("griddepcontrol.wait;" ::: "memory");       // the parts are written
-  const int border = blockIdx.x + 1;
-  const Shares shares(*p.all, p.grid);
-  if (border >= shares.owners) return;
-  const int4 here = p.starts[border], before = p.starts[border - 1];
-  if (here.z == 0) return;                                 // this run begins with its sequence
-  const bool same = before.x == here.x && before.y == here.y;
-  if (same && before.z > 0) return;                        // the run before begins inside the same sequence
-  const int kv = here.y / p.tiles, row0 = (here.y - kv * p.tiles) * 16, own = threadIdx.x >> 7, r = blockIdx.y * JOIN_ROWS + own;
-  const bool live = row0 + r < p.group && r < 16;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = threadIdx.x & 127;
-  // the parts: the last of the run before (its first, if that begins with this sequence), and the first of every run that begins
-  // in it, up to the owner of its last unit
-  const int parts = live ? shares.owner(shares.begin(border) - here.z + here.w - 1) - border + 2 : 0;
-  auto slot_of = [&](int i) { return ((long long)(border - 1 + i) * 2 + (i == 0 && !same ? 1 : 0)) * p.rows + r; };
-  float* w = weights + own * p.grid;
+  const int4 border = p.borders[blockIdx.x + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, own = warp / JOIN_WARPS, share = warp % JOIN_WARPS, r = blockIdx.y * JOIN_ROWS + own;
+  if (border.x == 0 || blockIdx.y * JOIN_ROWS >= border.w) return;
+  const int parts = r < border.w ? border.x : 0;
+  // the first part is border.y, the others are the first ones of the runs that follow
+  auto slot_of = [&](int i) { return ((long long)(i == 0 ? border.y : (border.y | 1) + 2 * i - 1) * p.rows + r); };
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
   float top = -INFINITY, sum = 0.f;
-  for (int i = t; i < parts; i += 128) { w[i] = p.part_ml[slot_of(i) * 2]; top = fmaxf(top, w[i]); }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) reduce[warp] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(reduce[own * 4], reduce[own * 4 + 1]), fmaxf(reduce[own * 4 + 2], reduce[own * 4 + 3]));
-  __syncthreads();
-  for (int i = t; i < parts; i += 128) {                   // a thread's own
-    w[i] = weight_of(w[i], top);
-    sum += w[i] * p.part_ml[slot_of(i) * 2 + 1];
+  for (int i = lane; i < parts; i += 32) {
+    const float2 x = ml[slot_of(i)];
+    const float higher = fmaxf(top, x.x);
+    sum = sum * weight_of(top, higher) + x.y * weight_of(x.x, higher);
+    top = higher;
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) reduce[warp] = sum;
-  __syncthreads();
-  sum = reduce[own * 4] + reduce[own * 4 + 1] + reduce[own * 4 + 2] + reduce[own * 4 + 3];
-  const int pair = t % (D / 2), share = t / (D / 2);
-  float2 y = make_float2(0.f, 0.f);
+  for (int o = 16; o > 0; o >>= 1) {
+    const float other = __shfl_xor_sync(0xffffffffu, top, o), more = __shfl_xor_sync(0xffffffffu, sum, o), higher = fmaxf(top, other);
+    sum = sum * weight_of(top, higher) + more * weight_of(other, higher);
+    top = higher;
+  }
+  Channels y = {};
 #pragma unroll 8
-  for (int i = share; i < parts; i += 256 / D) {
-    const float2 o = *reinterpret_cast<const float2*>(p.part_o + slot_of(i) * D + pair * 2);
-    y.x += w[i] * o.x;
-    y.y += w[i] * o.y;
-  }
-  sums[own][t] = y;
-  __syncthreads();
-  if (share || !live) return;
+  for (int i = share; i < parts; i += JOIN_WARPS) {
+    const Channels o = *reinterpret_cast<const Channels*>(p.part_o + slot_of(i) * D + lane * VEC);
+    const float w = weight_of(ml[slot_of(i)].x, top);
 #pragma unroll
-  for (int q = 1; q < 256 / D; ++q) { y.x += sums[own][q * (D / 2) + pair].x; y.y += sums[own][q * (D / 2) + pair].y; }
-  const long long head = (long long)here.x * p.hk * p.group + kv * p.group + row0 + r;
+    for (int j = 0; j < VEC; ++j) y.v[j] += w * o.v[j];
+  }
+  sums[own][share][lane] = y;
+  __syncthreads();
+  if (share || !parts) return;
+#pragma unroll
+  for (int q = 1; q < JOIN_WARPS; ++q)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) y.v[j] += sums[own][q][lane].v[j];
+  const long long head = border.z + r;
+  const int kv = (border.z / p.group) % p.hk;
   const float scale = sum == 0.f ? 0.f : (p.v_scale ? __ldg(p.v_scale + kv) : 1.f) / sum;
-  *reinterpret_cast<uint32_t*>(p.out + head * D + pair * 2) = sum == 0.f ? 0u : pack_bf16(y.x * scale, y.y * scale);
-  if (p.lse && pair == 0) p.lse[head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945f;
+#pragma unroll
+  for (int j = 0; j < VEC; j += 2)
+    *reinterpret_cast<uint32_t*>(p.out + head * D + lane * VEC + j) = sum == 0.f ? 0u : pack_bf16(y.v[j] * scale, y.v[j + 1] * scale);
+  if (p.lse && lane == 0) p.lse[head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945f;
 }
 
 // CTAs that run beside each other, for units of which there are at most `most`.
@@ -577,7 +581,6 @@ int launch(const Params& p, cudaStream_t stream) {
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(p.grid - 1, (p.rows + JOIN_ROWS - 1) / JOIN_ROWS);
   config.blockDim = dim3(JOIN_THREADS);
-  config.dynamicSmemBytes = p.grid * JOIN_ROWS * sizeof(float);
   config.stream = stream;
   cudaLaunchAttribute early;
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -594,7 +597,7 @@ bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_
 
 extern "C" size_t tw_paged_attention_workspace(int batch, int hq, int hk, int dim, long long tokens) {
   if (batch <= 0 || hk <= 0 || hq <= 0 || hq % hk || dim <= 0 || tokens < 0) return 0;
-  return (size_t)grid_of(batch, hq, hk, tokens) * (16 + 2 * part_rows(hq, hk) * (dim + 2) * 4) + 16;
+  return (size_t)grid_of(batch, hq, hk, tokens) * (16 + 2 * part_rows(hq, hk) * (dim + 2) * 4);
 }
 
 extern "C" int tw_paged_attention(const TwPagedAttentionArgs* a, void* stream) {
@@ -625,10 +628,9 @@ extern "C" int tw_paged_attention(const TwPagedAttentionArgs* a, void* stream) {
   p.pages = a->pages; p.max_pages = a->max_pages; p.rows = part_rows(a->hq, a->hk); p.grid = grid_of(a->batch, a->hq, a->hk, tokens);
   while ((1 << p.page_shift) < a->page) ++p.page_shift;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-  p.all = reinterpret_cast<int*>(ws);
-  p.starts = reinterpret_cast<int4*>(ws + 16);
-  p.part_ml = reinterpret_cast<float*>(p.starts + p.grid);
-  p.part_o = p.part_ml + (size_t)p.grid * 2 * p.rows * 2;
+  p.borders = reinterpret_cast<int4*>(ws);
+  p.part_ml = reinterpret_cast<float*>(p.borders + p.grid);
+  p.part_o = p.part_ml + (size_t)p.grid * 2 * p.rows * 2;                 // 16-byte aligned, as part_ml
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (p.rows <= 8) {
     if (a->dim == 128) return a->fp8 ? launch<128, true, false>(p, st) : launch<128, false, false>(p, st);
