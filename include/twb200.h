@@ -220,6 +220,40 @@ typedef struct TwPagedAttentionArgs {
 size_t tw_paged_attention_workspace(int batch, int hq, int hk, int dim, long long tokens);
 int tw_paged_attention(const TwPagedAttentionArgs* args, void* stream);
 
+/* ---- pages of a key-value cache ------------------------------------------------------------------
+ * State on the device: table [sequences, max_pages] (page numbers, -1 behind a sequence's pages), lengths [sequences] (tokens), refs
+ * [pages] (sequences that hold a page, 0: free). All calls are asynchronous and can be captured. append, fork and compact change
+ * nothing when they cannot be done, and raise *status to "a page table entry, slot or length leads outside the cache" or "the
+ * page pool or a sequence's table is full"; free leaves out what leads outside, and reports it. sequences <= 65536. */
+typedef struct TwCache {
+  void *k_pages, *v_pages;       /* [pages, hk, page, dim], rows contiguous, bf16 or (fp8) E4M3, 16-byte aligned heads */
+  int32_t *table, *lengths, *refs;
+  int32_t* status;               /* device word, or NULL */
+  long long k_stride_page, k_stride_head, v_stride_page, v_stride_head, table_stride; /* elements */
+  int32_t sequences, max_pages, pages, hk, page, dim, fp8;
+} TwCache;
+/* Rows cu[i] ... cu[i + 1] - 1 of k and v (row i when cu is NULL) go behind the tokens of slot slots[i] (i when slots is NULL); a slot may
+ * be named once. New pages are the lowest free numbers, in the order of i. fp8: rounded from k / k_scale[head], saturating. */
+typedef struct TwAppendArgs {
+  const void *k, *v;             /* bf16, row r, head h at k + r * k_stride_row + h * k_stride_head; strides multiples of 8 */
+  const int32_t *slots, *cu;     /* [batch] or NULL, [batch + 1] or NULL */
+  const float *k_scale, *v_scale;/* [hk] or NULL */
+  long long k_stride_row, k_stride_head, v_stride_row, v_stride_head;
+  int32_t batch, rows;
+} TwAppendArgs;
+size_t tw_cache_append_workspace(int batch, int rows);
+int tw_cache_append(const TwCache* cache, const TwAppendArgs* args, void* workspace, void* stream);
+/* children[i] (an empty slot, named once) becomes a copy of parents[i] as it was before the call: full pages are shared, the rows of a partly filled last page
+ * are copied to the lowest free page. */
+size_t tw_cache_fork_workspace(int count);
+int tw_cache_fork(const TwCache* cache, const int32_t* parents, const int32_t* children, int count, void* workspace, void* stream);
+/* Empties the slots: their pages lose a reference, their table entries become -1. Naming a slot twice is naming it once. */
+int tw_cache_free(const TwCache* cache, const int32_t* slots, int count, void* stream);
+/* Moves live pages to the numbers 0 ... live - 1: the r-th live page at or above `live` to the r-th free one below. *live (optional)
+ * receives their number. */
+size_t tw_cache_compact_workspace(int pages);
+int tw_cache_compact(const TwCache* cache, int32_t* live, void* workspace, void* stream);
+
 /* ---- pointwise producers with fused tensor factor ------------------------------------------
  * Each writes its bf16 result once and, when `stats` is given, reduces max|y| in the same pass:
  * stats[0] = factor = max|y| / 2688 (1.0 for an all-zero tensor, thunderworld_fp4/_linear_kernels.py:17-19

@@ -11,11 +11,21 @@ from .head_finding import config_from_head_scores, make_repair_mask, policy_from
 __version__ = '0.1.0'
 __all__ = ['PRESETS', 'RepairConfig', 'RepairPolicy', 'RepairRule', 'preset', 'fp4_attention', 'FP4Attention',
            'LinearRepairConfig', 'InferenceConfig', 'FP4Linear', 'Native', 'config_from_head_scores',
-           'make_repair_mask', 'policy_from_head_atlas']
+           'make_repair_mask', 'policy_from_head_atlas', 'PagedCache', 'paged_attention', 'fp4_matvec']
 
 
 def fp4_attention(*args, **kwargs):
     from .runtime import fp4_attention as implementation
+    return implementation(*args, **kwargs)
+
+
+def paged_attention(*args, **kwargs):
+    from .ops import paged_attention as implementation
+    return implementation(*args, **kwargs)
+
+
+def fp4_matvec(*args, **kwargs):
+    from .ops import fp4_matvec as implementation
     return implementation(*args, **kwargs)
 
 
@@ -29,4 +39,7 @@ def __getattr__(name):
     if name == 'Native':
         from .native import Native
         return Native
+    if name == 'PagedCache':
+        from .cache import PagedCache
+        return PagedCache
     raise AttributeError(name)

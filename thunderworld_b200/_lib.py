@@ -67,6 +67,17 @@ class PagedAttentionArgs(ctypes.Structure):
                [(n, _i) for n in ('batch', 'sequences', 'hq', 'hk', 'dim', 'page', 'pages', 'max_pages', 'fp8')]
 
 
+class Cache(ctypes.Structure):
+    _fields_ = [(n, _vp) for n in ('k_pages', 'v_pages', 'table', 'lengths', 'refs', 'status')] + \
+               [(n, _ll) for n in ('k_stride_page', 'k_stride_head', 'v_stride_page', 'v_stride_head', 'table_stride')] + \
+               [(n, _i) for n in ('sequences', 'max_pages', 'pages', 'hk', 'page', 'dim', 'fp8')]
+
+
+class AppendArgs(ctypes.Structure):
+    _fields_ = [(n, _vp) for n in ('k', 'v', 'slots', 'cu', 'k_scale', 'v_scale')] + \
+               [(n, _ll) for n in ('k_stride_row', 'k_stride_head', 'v_stride_row', 'v_stride_head')] + [(n, _i) for n in ('batch', 'rows')]
+
+
 _lib = None
 
 
@@ -117,6 +128,13 @@ def load():
     lib.tw_matvec.argtypes = [ctypes.POINTER(MatvecArgs), _vp]; lib.tw_matvec.restype = _i
     lib.tw_paged_attention_workspace.argtypes = [_i] * 4 + [_ll]; lib.tw_paged_attention_workspace.restype = ctypes.c_size_t
     lib.tw_paged_attention.argtypes = [ctypes.POINTER(PagedAttentionArgs), _vp]; lib.tw_paged_attention.restype = _i
+    for name, count in (('append', 2), ('fork', 1), ('compact', 1)):
+        getattr(lib, f'tw_cache_{name}_workspace').argtypes = [_i] * count
+        getattr(lib, f'tw_cache_{name}_workspace').restype = ctypes.c_size_t
+    lib.tw_cache_append.argtypes = [ctypes.POINTER(Cache), ctypes.POINTER(AppendArgs), _vp, _vp]; lib.tw_cache_append.restype = _i
+    lib.tw_cache_fork.argtypes = [ctypes.POINTER(Cache), _vp, _vp, _i, _vp, _vp]; lib.tw_cache_fork.restype = _i
+    lib.tw_cache_free.argtypes = [ctypes.POINTER(Cache), _vp, _i, _vp]; lib.tw_cache_free.restype = _i
+    lib.tw_cache_compact.argtypes = [ctypes.POINTER(Cache), _vp, _vp, _vp]; lib.tw_cache_compact.restype = _i
     _lib = lib
     return lib
 
@@ -136,4 +154,5 @@ EXPORTS = ('tw_status', 'tw_abi_version', 'tw_quantize_workspace', 'tw_quantize'
            'tw_workspace', 'tw_fused', 'tw_fused_tile_n', 'tw_pack_rows', 'tw_select_tiles', 'tw_attention',
            'tw_attention_workspace', 'tw_activate', 'tw_rms_norm', 'tw_rms_norm_heads', 'tw_rope_heads', 'tw_gate_residual',
            'tw_gate_residual_norm', 'tw_capture_id', 'tw_matvec',
-           'tw_paged_attention_workspace', 'tw_paged_attention')
+           'tw_paged_attention_workspace', 'tw_paged_attention', 'tw_cache_append_workspace', 'tw_cache_append', 'tw_cache_fork_workspace',
+           'tw_cache_fork', 'tw_cache_free', 'tw_cache_compact_workspace', 'tw_cache_compact')

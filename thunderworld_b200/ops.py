@@ -215,7 +215,8 @@ def fp4_matvec(x, codes, scales, factor, *, prescale=None, bias=None, wr=None, w
     y = factor * (bf16(x * prescale) @ W.T) + bias, W = codes [N, K/2] x E4M3 scales [N, K/16] plus the W1 tiles of a bank
     (wr [slots, 128, 64], wrs [slots, 128, 8]; wi, off, wloc, shared, dense as in fused_gemm), sums of 32 bits, one rounding.
     factor: float32 scalar tensor; prescale float32 [K]; bias bf16 [N]; out_dtype bfloat16 or float32. Any N, K a multiple of
-    32 up to 32768; with a bank both multiples of 128. One launch (two for more than 16 rows of a K above 21 k)."""
+    32 up to 32768; with a bank both multiples of 128. One launch (two for more rows of a K above 13 k than fit
+    an SM's shared memory)."""
     if x.ndim < 1 or x.dtype is not torch.bfloat16 or not x.is_cuda:
         raise ValueError('expected CUDA BF16 rows [..., K]')
     if codes.ndim != 2 or codes.dtype is not torch.uint8 or not codes.is_contiguous():
@@ -374,6 +375,99 @@ def paged_attention(q, k_pages, v_pages, table, lengths, *, slots=None, scale=No
             table.shape[0], hq, hk, dim, page, pages, table.shape[1], int(fp8))
         _lib.check(lib.tw_paged_attention(ctypes.byref(args), _stream(dev)))
     return (out, lse) if return_lse else out
+
+
+def _cache(k_pages, v_pages, table, lengths, refs, page=None):
+    """(argument struct, device, pool geometry) of a paged cache whose small tables are updated in place."""
+    if k_pages is not None:
+        pages, hk, page, dim, fp8 = _check_pages(k_pages, v_pages)
+        if (pages > 1 and not (k_pages.stride(0) and v_pages.stride(0))) or (hk > 1 and not (k_pages.stride(1) and v_pages.stride(1))):
+            raise ValueError('pages are written: they must not be expanded')
+        dev, strides = k_pages.device, (k_pages.stride(0), k_pages.stride(1), v_pages.stride(0), v_pages.stride(1))
+    else:
+        dev, pages, hk, dim, fp8, strides = refs.device, refs.numel(), 0, 0, False, (0, 0, 0, 0)
+        if type(page) is not int or page < 1 or page & (page - 1):
+            raise ValueError('tokens per page must be a power of two')
+    _check_table(dev, table, lengths)
+    if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+        raise ValueError('table is written: its rows must not overlap')
+    _check_int32(dev, refs=refs)
+    if refs.numel() != pages:
+        raise ValueError('refs must hold one count per page')
+    require_sm100(dev)
+    args = _lib.Cache(_ptr(k_pages), _ptr(v_pages), table.data_ptr(), lengths.data_ptr(), refs.data_ptr(), _cache_status(dev).data_ptr(), *strides,
+                      table.stride(0), table.shape[0], table.shape[1], pages, hk, page, dim, int(fp8))
+    return args, dev, (hk, dim, fp8)
+
+
+def cache_append_(k, v, k_pages, v_pages, table, lengths, refs, *, slots=None, cu=None, k_scale=None, v_scale=None):
+    """New tokens behind their sequences: rows k, v bf16 [rows, kv_heads, dim] go to the cache, row i behind the tokens of slot
+    slots[i] (i by default), or with cu int32 [batch + 1] rows cu[i] ... cu[i + 1] - 1. New pages are the lowest free numbers, in the
+    order of i; table, lengths and refs are updated. A slot may be named once. E4M3 pages hold k / k_scale[head] rounded, saturating.
+    All on the device: a call that cannot be done (a full pool or table, an index outside) changes nothing and shows in device_status()."""
+    args, dev, (hk, dim, fp8) = _cache(k_pages, v_pages, table, lengths, refs)
+    for t in (k, v):
+        if t.ndim != 3 or t.dtype is not torch.bfloat16 or t.device != dev or tuple(t.shape[1:]) != (hk, dim) or t.shape[0] != k.shape[0]:
+            raise ValueError('k and v must be BF16 [rows, kv_heads, dim] alike, on the device of the pages')
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+        raise RuntimeError('the cache is inference-only; use torch.inference_mode()')
+    _check_int32(dev, slots=slots, cu=cu)
+    _check_scales(dev, hk, k_scale, v_scale, fp8)
+    rows = k.shape[0]
+    batch = slots.numel() if slots is not None else (cu.numel() - 1 if cu is not None else rows)
+    if (cu is None and batch != rows) or (cu is not None and cu.numel() != batch + 1):
+        raise ValueError('one row per slot, or cu with one offset more than there are slots, is required')
+    if slots is None and batch > table.shape[0]:
+        raise ValueError('more entries than sequences')
+    if batch < 1 or not rows:
+        return
+    laid = [t if t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0
+            else t.clone(memory_format=torch.contiguous_format) for t in (k, v)]
+    call = _lib.AppendArgs(laid[0].data_ptr(), laid[1].data_ptr(), _ptr(slots), _ptr(cu), _ptr(k_scale), _ptr(v_scale), laid[0].stride(0),
+                           laid[0].stride(1), laid[1].stride(0), laid[1].stride(1), batch, rows)
+    lib = _lib.load()
+    with _device(dev):
+        scratch = torch.empty(lib.tw_cache_append_workspace(batch, rows), device=dev, dtype=torch.uint8)
+        _lib.check(lib.tw_cache_append(ctypes.byref(args), ctypes.byref(call), scratch.data_ptr(), _stream(dev)))
+
+
+def cache_fork_(k_pages, v_pages, table, lengths, refs, parents, children):
+    """Slot children[i], which must be empty and may be named once, becomes a copy of slot parents[i] as it was before the call: full
+    pages are shared (refs counts their holders), the rows of a partly filled last page are copied to the lowest free page. int32 [n] each. A call that cannot be
+    done changes nothing and shows in device_status()."""
+    args, dev, _ = _cache(k_pages, v_pages, table, lengths, refs)
+    _check_int32(dev, parents=parents, children=children)
+    count = parents.numel()
+    if children.numel() != count:
+        raise ValueError('one child per parent is required')
+    if not count:
+        return
+    lib = _lib.load()
+    with _device(dev):
+        scratch = torch.empty(lib.tw_cache_fork_workspace(count), device=dev, dtype=torch.uint8)
+        _lib.check(lib.tw_cache_fork(ctypes.byref(args), parents.data_ptr(), children.data_ptr(), count, scratch.data_ptr(), _stream(dev)))
+
+
+def cache_free_(table, lengths, refs, slots, page_size):
+    """Empties slots int32 [n] of a cache with page_size tokens per page: their pages lose a reference, their table entries become -1. A
+    slot named twice is freed once; one outside is left out and shows in device_status()."""
+    args, dev, _ = _cache(None, None, table, lengths, refs, page_size)
+    _check_int32(dev, slots=slots)
+    if slots.numel():
+        with _device(dev):
+            _lib.check(_lib.load().tw_cache_free(ctypes.byref(args), slots.data_ptr(), slots.numel(), _stream(dev)))
+
+
+def cache_compact_(k_pages, v_pages, table, lengths, refs):
+    """Moves the live pages to the numbers 0 ... live - 1 (the r-th live page at or above live to the r-th free one below), updates table
+    and refs, and returns live as an int32 scalar tensor."""
+    args, dev, _ = _cache(k_pages, v_pages, table, lengths, refs)
+    live = torch.empty((), device=dev, dtype=torch.int32)
+    lib = _lib.load()
+    with _device(dev):
+        scratch = torch.empty(lib.tw_cache_compact_workspace(refs.numel()), device=dev, dtype=torch.uint8)
+        _lib.check(lib.tw_cache_compact(ctypes.byref(args), live.data_ptr(), scratch.data_ptr(), _stream(dev)))
+    return live
 
 
 STATUS_KEYS = {'g': 0, 'a': 0, 'q': 8, 'c': 0}   # workspace -> byte offset of its device status word: fused GEMM, attention, quantizer, paged cache
