@@ -188,11 +188,14 @@ class DiTBlock(torch.nn.Module):
         ops.gate_residual_(x_rows.unsqueeze(0), gate2, part.unsqueeze(0))
         return x_rows
 
-    def forward(self, x, mod):
-        """x bf16 [batch, tokens, hidden], updated in place; mod [6, batch, hidden] contiguous."""
+    def forward(self, x, mod, entry=None, following=None):
+        """x bf16 [batch, tokens, hidden], updated in place; mod [6, batch, hidden] contiguous. A residual and the norm behind it are
+        one pass (the bits of gate_residual_ followed by rms_norm): `entry` is this block's first norm and its factor, where the
+        block before has made them, and `following` the modulation (shift, scale) of the norm behind this block, (None, None) for a
+        plain one; the call then returns that norm and its factor instead of x."""
         b, s, h = x.shape
         shift1, scale1, gate1, shift2, scale2, gate2 = mod.unbind(0)
-        y, f = ops.rms_norm(x, shift=shift1, scale=scale1, want_factor=True)
+        y, f = ops.rms_norm(x, shift=shift1, scale=scale1, want_factor=True) if entry is None else entry
         qkv = self.qkv(y, factor=f).reshape(b, s, 3, self.local_heads, 128)
         q, k, v = qkv.unbind(2)
         if self.cfg.rope:
@@ -204,10 +207,12 @@ class DiTBlock(torch.nn.Module):
         elif self.cfg.qk_norm:
             q, k = ops.rms_norm_heads(q), ops.rms_norm_heads(k)
         a = self.controller.attend(self.index, q, k, v).reshape(b, s, self.local_heads * 128)
-        ops.gate_residual_(x, gate1, self._row_split(self.out, a))
-        y, f = ops.rms_norm(x, shift=shift2, scale=scale2, want_factor=True)
+        y, f = ops.gate_residual_norm_(x, self._row_split(self.out, a), gate1, shift=shift2, scale=scale2, want_factor=True)
         u, stats = self.up(y, factor=f, activation='gelu_tanh')      # GELU and max|u| come out of the GEMM epilogue
-        return ops.gate_residual_(x, gate2, self._row_split(self.down, u, stats))
+        down = self._row_split(self.down, u, stats)
+        if following is None:
+            return ops.gate_residual_(x, gate2, down)
+        return ops.gate_residual_norm_(x, down, gate2, shift=following[0], scale=following[1], want_factor=True)
 
 
 class DiTModel(torch.nn.Module):
@@ -237,6 +242,10 @@ class DiTModel(torch.nn.Module):
             parallel.all_gather_rows([(full, mine)], topo)
             return full[:tokens].unsqueeze(0)
         x = x.clone()                                         # blocks update the residual stream in place
+        if not len(self.blocks):
+            return ops.rms_norm(x)
+        entry = None
         for i, block in enumerate(self.blocks):
-            x = block(x, mods[i])
-        return ops.rms_norm(x)
+            following = (mods[i + 1, 0], mods[i + 1, 1]) if i + 1 < len(self.blocks) else (None, None)
+            entry = block(x, mods[i], entry, following)
+        return entry[0]
