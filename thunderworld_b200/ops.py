@@ -12,6 +12,7 @@ torch is used for device memory and streams only.
 import ctypes
 from contextlib import nullcontext
 from dataclasses import dataclass
+from functools import lru_cache
 import torch
 from . import _lib
 
@@ -280,56 +281,71 @@ def fp4_matvec(x, codes, scales, factor, *, prescale=None, bias=None, wr=None, w
 
 
 # ---- paged key-value cache --------------------------------------------------------------------------
+_status_words = {}
+
+
 def _cache_status(device):
-    """The device word that the paged operators report in (device_status reads it)."""
-    word = _workspaces.get((device, 'c'))
+    """Address of the device word that the paged operators report in (device_status reads it; it lives as long as the process)."""
+    word = _status_words.get(device)
     if word is None:
-        word = _workspace(device, 256, 'c')
+        word = _workspace(device, 256, 'c').data_ptr()
         if not torch.cuda.is_current_stream_capturing():
             torch.cuda.current_stream(device).synchronize()       # zeroed before another stream's call may write it
+        _status_words[device] = word
     return word
 
 
 def _check_pages(k_pages, v_pages):
-    """(pages, kv heads, page, dim, fp8) of the two halves of a pool; raises where they are not pages."""
-    if k_pages.ndim != 4 or k_pages.shape != v_pages.shape or not k_pages.numel():
+    """(pages, kv heads, page, dim, fp8, strides of k, of v) of the two halves of a pool; raises where they are not pages."""
+    shape, dtype = k_pages.shape, k_pages.dtype
+    if len(shape) != 4 or shape != v_pages.shape or not k_pages.numel():
         raise ValueError('k_pages and v_pages must be [pages, kv_heads, page, dim] alike')
-    if k_pages.dtype is not v_pages.dtype or (k_pages.dtype is not torch.bfloat16 and k_pages.dtype is not torch.float8_e4m3fn):
+    if dtype is not v_pages.dtype or (dtype is not torch.bfloat16 and dtype is not torch.float8_e4m3fn):
         raise ValueError('pages must be bfloat16 or float8_e4m3fn')
-    pages, hk, page, dim = k_pages.shape
+    pages, hk, page, dim = shape
     if dim != 64 and dim != 128:
         raise ValueError('head dimension must be 64 or 128')
     if page & (page - 1):
         raise ValueError('tokens per page must be a power of two')
-    for t in (k_pages, v_pages):
-        if t.stride(3) != 1 or (page > 1 and t.stride(2) != dim):
-            raise ValueError('the rows of a page must lie one behind the other')
+    ks, vs = k_pages.stride(), v_pages.stride()
+    if ks[3] != 1 or vs[3] != 1 or (page > 1 and (ks[2] != dim or vs[2] != dim)):
+        raise ValueError('the rows of a page must lie one behind the other')
     if not k_pages.is_cuda or v_pages.device != k_pages.device:
         raise ValueError('pages must be on one CUDA device')
-    return pages, hk, page, dim, k_pages.dtype is torch.float8_e4m3fn
+    return pages, hk, page, dim, dtype is torch.float8_e4m3fn, ks, vs
 
 
-def _check_int32(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and (t.dtype is not torch.int32 or t.device != device or t.ndim != 1 or (t.numel() > 1 and t.stride(0) != 1)):
-            raise ValueError(f'{name} must be contiguous int32 on the device of the pages')
+def _check_int32(device, name, t):
+    if t is not None and (t.dtype is not torch.int32 or t.ndim != 1 or t.device != device or (t.stride(0) != 1 and t.numel() > 1)):
+        raise ValueError(f'{name} must be contiguous int32 on the device of the pages')
 
 
 def _check_table(device, table, lengths):
-    if table.ndim != 2 or table.dtype is not torch.int32 or table.device != device or not table.numel() or table.stride(1) != 1:
+    """(sequences, pages per sequence, row stride) of a page table."""
+    if table.ndim != 2 or table.dtype is not torch.int32 or table.device != device or not table.numel():
         raise ValueError('table must be int32 [sequences, pages per sequence] with contiguous rows, on the device of the pages')
-    _check_int32(device, lengths=lengths)
-    if lengths.numel() != table.shape[0]:
+    (sequences, width), strides = table.shape, table.stride()
+    if strides[1] != 1:
+        raise ValueError('table must be int32 [sequences, pages per sequence] with contiguous rows, on the device of the pages')
+    _check_int32(device, 'lengths', lengths)
+    if lengths.numel() != sequences:
         raise ValueError('lengths must hold one entry per row of table')
+    return sequences, width, strides[0]
 
 
 def _check_scales(device, hk, k_scale, v_scale, fp8):
+    if k_scale is None and v_scale is None:
+        return
+    if not fp8:
+        raise ValueError('scales come with float8_e4m3fn pages')
     for name, t in (('k_scale', k_scale), ('v_scale', v_scale)):
-        if t is not None:
-            if not fp8:
-                raise ValueError('scales come with float8_e4m3fn pages')
-            if t.dtype is not torch.float32 or t.device != device or tuple(t.shape) != (hk,) or not t.is_contiguous():
-                raise ValueError(f'{name} must be contiguous float32 [kv_heads] on the device of the pages')
+        if t is not None and (t.dtype is not torch.float32 or t.device != device or tuple(t.shape) != (hk,) or not t.is_contiguous()):
+            raise ValueError(f'{name} must be contiguous float32 [kv_heads] on the device of the pages')
+
+
+@lru_cache(maxsize=4096)
+def _scratch_bytes(name, *sizes):
+    return getattr(_lib.load(), name)(*sizes)
 
 
 def paged_attention(q, k_pages, v_pages, table, lengths, *, slots=None, scale=None, k_scale=None, v_scale=None, return_lse=False, out=None):
@@ -341,63 +357,65 @@ def paged_attention(q, k_pages, v_pages, table, lengths, *, slots=None, scale=No
     no host synchronisation. scale defaults to dim ** -0.5. Returns bf16 [batch, heads, dim], with return_lse also the float32
     natural log of each softmax's sum (-inf and zeros for an empty sequence). Sums are 32 bits wide. Slots, lengths and table entries
     that lead outside are left out and reported by device_status()."""
-    pages, hk, page, dim, fp8 = _check_pages(k_pages, v_pages)
+    pages, hk, page, dim, fp8, ks, vs = _check_pages(k_pages, v_pages)
     dev = k_pages.device
     if q.ndim != 3 or q.dtype is not torch.bfloat16 or q.device != dev or q.shape[2] != dim or q.stride(2) != 1:
         raise ValueError('q must be BF16 [batch, heads, dim] with contiguous rows, on the device of the pages')
-    batch, hq = q.shape[0], q.shape[1]
+    shape = q.shape
+    batch, hq, _ = shape
     if not batch or not hq or hq % hk:
         raise ValueError('a nonempty batch and a whole number of heads per kv head are required')
-    _check_table(dev, table, lengths)
-    _check_int32(dev, slots=slots)
-    if (batch if slots is None else slots.numel()) != batch or (slots is None and batch > table.shape[0]):
+    sequences, width, table_stride = _check_table(dev, table, lengths)
+    if slots is not None:
+        _check_int32(dev, 'slots', slots)
+    if (batch > sequences) if slots is None else (slots.numel() != batch):
         raise ValueError('slots must name one sequence per row of q')
     _check_scales(dev, hk, k_scale, v_scale, fp8)
-    if torch.is_grad_enabled() and q.requires_grad:
+    if q.requires_grad and torch.is_grad_enabled():
         raise RuntimeError('paged_attention is inference-only; use torch.inference_mode()')
     require_sm100(dev)
-    if q.data_ptr() % 4 or q.stride(0) % 2 or q.stride(1) % 2:
-        q = q.contiguous() if not q.is_contiguous() else q.clone()
-    shape = (batch, hq, dim)
+    qs = q.stride()
+    if qs[0] % 2 or qs[1] % 2 or q.data_ptr() % 4:
+        q = q.clone(memory_format=torch.contiguous_format)
+        qs = q.stride()
     if out is None:
         out = torch.empty(shape, device=dev, dtype=torch.bfloat16)
-    elif tuple(out.shape) != shape or out.dtype is not torch.bfloat16 or not out.is_contiguous() or out.device != dev:
-        raise ValueError(f'out must be contiguous BF16 {shape} on the device of the pages')
+    elif out.shape != shape or out.dtype is not torch.bfloat16 or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f'out must be contiguous BF16 {tuple(shape)} on the device of the pages')
     lse = torch.empty((batch, hq), device=dev, dtype=torch.float32) if return_lse else None
     lib = _lib.load()
     with _device(dev):
         # scratch of the call's own: calls on several streams, and captured ones, do not share it
-        scratch = torch.empty(lib.tw_paged_attention_workspace(batch, hq, hk, dim, table.shape[1] * page), device=dev, dtype=torch.uint8)
+        scratch = torch.empty(_scratch_bytes('tw_paged_attention_workspace', batch, hq, hk, dim, width * page), device=dev, dtype=torch.uint8)
         args = _lib.PagedAttentionArgs(
-            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lengths.data_ptr(), _ptr(slots), _ptr(k_scale), _ptr(v_scale),
-            out.data_ptr(), _ptr(lse), scratch.data_ptr(), _cache_status(dev).data_ptr(), q.stride(0), q.stride(1), k_pages.stride(0),
-            k_pages.stride(1), v_pages.stride(0), v_pages.stride(1), table.stride(0), dim ** -.5 if scale is None else float(scale), batch,
-            table.shape[0], hq, hk, dim, page, pages, table.shape[1], int(fp8))
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lengths.data_ptr(), None if slots is None else slots.data_ptr(),
+            _ptr(k_scale), _ptr(v_scale), out.data_ptr(), None if lse is None else lse.data_ptr(), scratch.data_ptr(), _cache_status(dev), qs[0], qs[1],
+            ks[0], ks[1], vs[0], vs[1], table_stride, dim ** -.5 if scale is None else scale, batch, sequences, hq, hk, dim, page, pages, width, fp8)
         _lib.check(lib.tw_paged_attention(ctypes.byref(args), _stream(dev)))
     return (out, lse) if return_lse else out
 
 
 def _cache(k_pages, v_pages, table, lengths, refs, page=None):
-    """(argument struct, device, pool geometry) of a paged cache whose small tables are updated in place."""
+    """(argument struct, device, kv heads, dim, fp8, sequences) of a paged cache whose small tables are updated in place."""
     if k_pages is not None:
-        pages, hk, page, dim, fp8 = _check_pages(k_pages, v_pages)
-        if (pages > 1 and not (k_pages.stride(0) and v_pages.stride(0))) or (hk > 1 and not (k_pages.stride(1) and v_pages.stride(1))):
+        pages, hk, page, dim, fp8, ks, vs = _check_pages(k_pages, v_pages)
+        if (pages > 1 and not (ks[0] and vs[0])) or (hk > 1 and not (ks[1] and vs[1])):
             raise ValueError('pages are written: they must not be expanded')
-        dev, strides = k_pages.device, (k_pages.stride(0), k_pages.stride(1), v_pages.stride(0), v_pages.stride(1))
+        dev, pointers = k_pages.device, (k_pages.data_ptr(), v_pages.data_ptr())
     else:
-        dev, pages, hk, dim, fp8, strides = refs.device, refs.numel(), 0, 0, False, (0, 0, 0, 0)
+        dev, pages, hk, dim, fp8, ks, vs, pointers = refs.device, refs.numel(), 0, 0, False, (0, 0), (0, 0), (None, None)
         if type(page) is not int or page < 1 or page & (page - 1):
             raise ValueError('tokens per page must be a power of two')
-    _check_table(dev, table, lengths)
-    if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+    sequences, width, table_stride = _check_table(dev, table, lengths)
+    if sequences > 1 and table_stride < width:
         raise ValueError('table is written: its rows must not overlap')
-    _check_int32(dev, refs=refs)
+    _check_int32(dev, 'refs', refs)
     if refs.numel() != pages:
         raise ValueError('refs must hold one count per page')
     require_sm100(dev)
-    args = _lib.Cache(_ptr(k_pages), _ptr(v_pages), table.data_ptr(), lengths.data_ptr(), refs.data_ptr(), _cache_status(dev).data_ptr(), *strides,
-                      table.stride(0), table.shape[0], table.shape[1], pages, hk, page, dim, int(fp8))
-    return args, dev, (hk, dim, fp8)
+    args = _lib.Cache(*pointers, table.data_ptr(), lengths.data_ptr(), refs.data_ptr(), _cache_status(dev), ks[0], ks[1], vs[0], vs[1], table_stride,
+                      sequences, width, pages, hk, page, dim, fp8)
+    return args, dev, hk, dim, fp8, sequences
 
 
 def cache_append_(k, v, k_pages, v_pages, table, lengths, refs, *, slots=None, cu=None, k_scale=None, v_scale=None):
@@ -405,54 +423,59 @@ def cache_append_(k, v, k_pages, v_pages, table, lengths, refs, *, slots=None, c
     slots[i] (i by default), or with cu int32 [batch + 1] rows cu[i] ... cu[i + 1] - 1. New pages are the lowest free numbers, in the
     order of i; table, lengths and refs are updated. A slot may be named once. E4M3 pages hold k / k_scale[head] rounded, saturating.
     All on the device: a call that cannot be done (a full pool or table, an index outside) changes nothing and shows in device_status()."""
-    args, dev, (hk, dim, fp8) = _cache(k_pages, v_pages, table, lengths, refs)
-    for t in (k, v):
-        if t.ndim != 3 or t.dtype is not torch.bfloat16 or t.device != dev or tuple(t.shape[1:]) != (hk, dim) or t.shape[0] != k.shape[0]:
-            raise ValueError('k and v must be BF16 [rows, kv_heads, dim] alike, on the device of the pages')
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+    args, dev, hk, dim, fp8, sequences = _cache(k_pages, v_pages, table, lengths, refs)
+    shape = k.shape
+    if len(shape) != 3 or shape != v.shape or shape[1] != hk or shape[2] != dim or k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 \
+            or k.device != dev or v.device != dev:
+        raise ValueError('k and v must be BF16 [rows, kv_heads, dim] alike, on the device of the pages')
+    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         raise RuntimeError('the cache is inference-only; use torch.inference_mode()')
-    _check_int32(dev, slots=slots, cu=cu)
+    _check_int32(dev, 'slots', slots)
+    _check_int32(dev, 'cu', cu)
     _check_scales(dev, hk, k_scale, v_scale, fp8)
-    rows = k.shape[0]
+    rows = shape[0]
     batch = slots.numel() if slots is not None else (cu.numel() - 1 if cu is not None else rows)
     if (cu is None and batch != rows) or (cu is not None and cu.numel() != batch + 1):
         raise ValueError('one row per slot, or cu with one offset more than there are slots, is required')
-    if slots is None and batch > table.shape[0]:
+    if slots is None and batch > sequences:
         raise ValueError('more entries than sequences')
     if batch < 1 or not rows:
         return
-    laid = [t if t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0
-            else t.clone(memory_format=torch.contiguous_format) for t in (k, v)]
-    call = _lib.AppendArgs(laid[0].data_ptr(), laid[1].data_ptr(), _ptr(slots), _ptr(cu), _ptr(k_scale), _ptr(v_scale), laid[0].stride(0),
-                           laid[0].stride(1), laid[1].stride(0), laid[1].stride(1), batch, rows)
-    lib = _lib.load()
+    ks, vs = k.stride(), v.stride()
+    if ks[2] != 1 or ks[0] % 8 or ks[1] % 8 or k.data_ptr() % 16:
+        k = k.clone(memory_format=torch.contiguous_format)
+        ks = k.stride()
+    if vs[2] != 1 or vs[0] % 8 or vs[1] % 8 or v.data_ptr() % 16:
+        v = v.clone(memory_format=torch.contiguous_format)
+        vs = v.stride()
+    call = _lib.AppendArgs(k.data_ptr(), v.data_ptr(), _ptr(slots), _ptr(cu), _ptr(k_scale), _ptr(v_scale), ks[0], ks[1], vs[0], vs[1], batch, rows)
     with _device(dev):
-        scratch = torch.empty(lib.tw_cache_append_workspace(batch, rows), device=dev, dtype=torch.uint8)
-        _lib.check(lib.tw_cache_append(ctypes.byref(args), ctypes.byref(call), scratch.data_ptr(), _stream(dev)))
+        scratch = torch.empty(_scratch_bytes('tw_cache_append_workspace', batch, rows), device=dev, dtype=torch.uint8)
+        _lib.check(_lib.load().tw_cache_append(ctypes.byref(args), ctypes.byref(call), scratch.data_ptr(), _stream(dev)))
 
 
 def cache_fork_(k_pages, v_pages, table, lengths, refs, parents, children):
     """Slot children[i], which must be empty and may be named once, becomes a copy of slot parents[i] as it was before the call: full
     pages are shared (refs counts their holders), the rows of a partly filled last page are copied to the lowest free page. int32 [n] each. A call that cannot be
     done changes nothing and shows in device_status()."""
-    args, dev, _ = _cache(k_pages, v_pages, table, lengths, refs)
-    _check_int32(dev, parents=parents, children=children)
+    args, dev, *_ = _cache(k_pages, v_pages, table, lengths, refs)
+    _check_int32(dev, 'parents', parents)
+    _check_int32(dev, 'children', children)
     count = parents.numel()
     if children.numel() != count:
         raise ValueError('one child per parent is required')
     if not count:
         return
-    lib = _lib.load()
     with _device(dev):
-        scratch = torch.empty(lib.tw_cache_fork_workspace(count), device=dev, dtype=torch.uint8)
-        _lib.check(lib.tw_cache_fork(ctypes.byref(args), parents.data_ptr(), children.data_ptr(), count, scratch.data_ptr(), _stream(dev)))
+        scratch = torch.empty(_scratch_bytes('tw_cache_fork_workspace', count), device=dev, dtype=torch.uint8)
+        _lib.check(_lib.load().tw_cache_fork(ctypes.byref(args), parents.data_ptr(), children.data_ptr(), count, scratch.data_ptr(), _stream(dev)))
 
 
 def cache_free_(table, lengths, refs, slots, page_size):
     """Empties slots int32 [n] of a cache with page_size tokens per page: their pages lose a reference, their table entries become -1. A
     slot named twice is freed once; one outside is left out and shows in device_status()."""
-    args, dev, _ = _cache(None, None, table, lengths, refs, page_size)
-    _check_int32(dev, slots=slots)
+    args, dev, *_ = _cache(None, None, table, lengths, refs, page_size)
+    _check_int32(dev, 'slots', slots)
     if slots.numel():
         with _device(dev):
             _lib.check(_lib.load().tw_cache_free(ctypes.byref(args), slots.data_ptr(), slots.numel(), _stream(dev)))
@@ -461,12 +484,11 @@ def cache_free_(table, lengths, refs, slots, page_size):
 def cache_compact_(k_pages, v_pages, table, lengths, refs):
     """Moves the live pages to the numbers 0 ... live - 1 (the r-th live page at or above live to the r-th free one below), updates table
     and refs, and returns live as an int32 scalar tensor."""
-    args, dev, _ = _cache(k_pages, v_pages, table, lengths, refs)
+    args, dev, *_ = _cache(k_pages, v_pages, table, lengths, refs)
     live = torch.empty((), device=dev, dtype=torch.int32)
-    lib = _lib.load()
     with _device(dev):
-        scratch = torch.empty(lib.tw_cache_compact_workspace(refs.numel()), device=dev, dtype=torch.uint8)
-        _lib.check(lib.tw_cache_compact(ctypes.byref(args), live.data_ptr(), scratch.data_ptr(), _stream(dev)))
+        scratch = torch.empty(_scratch_bytes('tw_cache_compact_workspace', refs.numel()), device=dev, dtype=torch.uint8)
+        _lib.check(_lib.load().tw_cache_compact(ctypes.byref(args), live.data_ptr(), scratch.data_ptr(), _stream(dev)))
     return live
 
 
