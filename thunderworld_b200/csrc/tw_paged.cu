@@ -2,12 +2,12 @@
 //   o[b, h] = sum_t softmax_t(scale q[b, h] . k_t) v_t,  t < lengths[slot b],  k_t = k_pages[table[slot, t / page], h / G, t % page]
 // for G = hq / hk query heads per key head, head dimension 64 or 128, pages in bf16 or in E4M3 with a scale per key head.
 //
-// What bounds it is the read of the keys and values, once. The work is cut into units of 64 tokens of one (sequence, key head), in
-// that order, and the units are shared evenly by the CTAs that run beside each other, whatever the lengths (which only the device
+// What bounds it is the read of the keys and values, once. The work is cut into units of 64 tokens of one (sequence, key head), 128
+// where a row is shorter than 256 bytes, in that order, and the units are shared evenly by the CTAs that run beside each other, whatever the lengths (which only the device
 // knows; putting the warps' parts of a sequence together costs about a unit and is counted as one): a CTA's run may begin and end inside a sequence, and what it has of such a one goes to the workspace, unnormalised, with
 // its maximum and sum; a second small launch joins these in their order. A call needs no zeroed state and no counter, so calls
 // on several streams, and captured ones, do not meet.
-// A warp takes 16 of a unit's tokens: it copies their rows (two units ahead) to a ring of its own, multiplies q (the group's heads,
+// A warp takes 16 (32) of a unit's tokens: it copies their rows (two units ahead) to a ring of its own, multiplies q (the group's heads,
 // padded to 16 rows) by the keys, keeps its own running maximum and sum in 32 bits, base 2, and multiplies the probabilities
 // by the values on the tensor cores (m16n8k16, 32-bit sums); warps meet only at the end of a sequence. With bf16 pages a
 // probability is two bf16 values (8 + 8 bits), so that rounding it adds nothing to the result's own rounding (an infinite value
@@ -21,7 +21,9 @@
 
 namespace {
 
-constexpr int WARPS = 4, THREADS = WARPS * 32, UNIT = WARPS * 16;     // tokens of a unit
+constexpr int WARPS = 4, THREADS = WARPS * 32;
+// Tokens of a warp's tile: 16 of 256-byte rows, 32 of shorter ones (the instructions beside the products are per tile).
+__host__ __device__ constexpr int tile_tokens(int row_bytes) { return row_bytes >= 256 ? 16 : 32; }
 constexpr int JOIN_ROWS = 4;        // query rows that a CTA's warps put together at a time
 
 struct Params {
@@ -48,7 +50,6 @@ __device__ __forceinline__ int tokens_of(const Params& p, int b, int& slot) {
   if (n < 0 || n > most) { report(p); return n < 0 ? 0 : (int)most; }
   return n;
 }
-__device__ __forceinline__ int units_of(int tokens) { return (tokens + UNIT - 1) / UNIT; }
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
@@ -110,14 +111,17 @@ struct Cursor {
 // WIDE: more than 8 query rows per tile; else the lower half of the 16 rows is all there is, and nothing is computed for the rest.
 template <int D, bool FP8, bool WIDE>
 __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __grid_constant__ Params p) {
-  constexpr int ROW = D * (FP8 ? 1 : 2), CHUNKS = ROW / 16, TILE = 16 * ROW;      // bytes of a row, of 16 rows
+  constexpr int ROW = D * (FP8 ? 1 : 2), CHUNKS = ROW / 16, TOK = tile_tokens(ROW), SUBS = TOK / 16, UNIT = WARPS * TOK;
+  constexpr int SUB = 16 * ROW, TILE = SUBS * SUB;         // bytes of 16 tokens' rows, of a tile's
+  constexpr uint32_t ALL = TOK == 32 ? 0xffffffffu : 0xffffu;
   constexpr int STAGES = 2, HALVES = WIDE ? 2 : 1;
-  extern __shared__ __align__(128) uint8_t dynamic[];                             // [WARPS][STAGES][K, V][16 rows], from a multiple of 256
+  extern __shared__ __align__(128) uint8_t dynamic[];                             // [WARPS][STAGES][K, V][TOK rows], from a multiple of 256
   __shared__ float gather[WARPS * JOIN_ROWS * D];
   __shared__ float part_m[WARPS][16], part_l[WARPS][16];
   __shared__ float2 joined[16];
   __shared__ int sums[WARPS + 1], start_b, start_offset;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  auto units_of = [](int tokens) { return (tokens + UNIT - 1) / UNIT; };
 
   // ---- this CTA's run: the lengths' prefix sums, in units -----------------------------------------------------------
   const int per = (p.batch + THREADS - 1) / THREADS, first_b = min(threadIdx.x * per, p.batch), last_b = min(first_b + per, p.batch);
@@ -176,7 +180,7 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
   };
   auto advance = [&](Cursor& c) { --c.left; ++c.tile; settle(c); };
 
-  // ---- copies: 16 tokens' rows of K and of V to the warp's ring ---------------------------------------------
+  // ---- copies: a tile's rows of K and of V to the warp's ring ---------------------------------------------
   // rows begin at multiples of 256, so that a chunk's place in its row can be had by exclusive or
   const uint32_t ring = ((tw::smem_u32(dynamic) + 255) & ~255u) + warp * STAGES * 2 * TILE;
   constexpr int LANES = CHUNKS, STEP = 32 / LANES, COPIES = 16 / STEP;            // lanes per row, rows per instruction
@@ -210,10 +214,15 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
     p.borders[blockIdx.x] = border;
   }
   const int in_page = (1 << p.page_shift) - 1;
-  int next_page = 0;                   // where the tokens lie that are fetched next: looked up a tile ahead
+  int next_page[SUBS];                 // where the tokens lie that are fetched next: looked up a tile ahead
   auto look_up = [&]() {
-    const int t0 = in.tile * UNIT + warp * 16;
-    if (p.page_shift >= 4 && t0 < in.of->tokens) next_page = __ldg(p.table + in.of->slot * p.table_stride + (t0 >> p.page_shift));
+    const int t0 = (in.tile * WARPS + warp) * TOK;
+#pragma unroll
+    for (int u = 0; u < SUBS; ++u) {
+      next_page[u] = 0;
+      if (p.page_shift >= 4 && t0 + u * 16 < in.of->tokens)
+        next_page[u] = __ldg(p.table + in.of->slot * p.table_stride + ((t0 + u * 16) >> p.page_shift));
+    }
   };
   look_up();
   // the queries of the sequence entered, to where they are had quickly when its turn comes: a line per lane
@@ -224,46 +233,53 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
   };
   // Starts the copies of the next tile; returns which of its tokens count.
   auto fetch = [&](uint32_t to) -> uint32_t {
-    uint32_t mask = 0;
-    const int t0 = in.tile * UNIT + warp * 16;
+    uint32_t all_mask = 0;
+    const int t0 = (in.tile * WARPS + warp) * TOK;
     if (in.left > 0 && t0 < in.of->tokens) {
-      const int live = min(in.of->tokens - t0, 16), kv = in.of->kv;
-      if (p.page_shift >= 4) {         // the 16 tokens lie in one page, one behind the other
-        const bool inside = next_page >= 0 && next_page < p.pages;
-        if (!inside && lane == 0) report(p);
-        const long long page = inside ? next_page : 0, row = (long long)(t0 & in_page) * ROW + lane * 16;
-        const uint8_t *k = p.k + page * p.k_page + kv * p.k_head + row, *v = p.v + page * p.v_page + kv * p.v_head + row;
-        if (inside) mask = 0xffffu >> (16 - live);
-        if (mask == 0xffffu) {
+      const int kv = in.of->kv, left = in.of->tokens - t0;
 #pragma unroll
-          for (int i = 0; i < COPIES; ++i) {
-            copy16(to + place[i % PLACES] + i * 512, k + i * 512);
-            copy16(to + TILE + place[i % PLACES] + i * 512, v + i * 512);
+      for (int u = 0; u < SUBS; ++u) {
+        const int live = min(left - u * 16, 16);
+        uint32_t mask = 0;
+        const uint32_t sub = to + u * SUB;
+        if (p.page_shift >= 4) {       // 16 tokens lie in one page, one behind the other
+          const bool inside = next_page[u] >= 0 && next_page[u] < p.pages;
+          if (!inside && lane == 0) report(p);
+          const long long page = inside ? next_page[u] : 0, row = (long long)((t0 + u * 16) & in_page) * ROW + lane * 16;
+          const uint8_t *k = p.k + page * p.k_page + kv * p.k_head + row, *v = p.v + page * p.v_page + kv * p.v_head + row;
+          if (inside && live > 0) mask = 0xffffu >> (16 - live);
+          if (mask == 0xffffu) {
+#pragma unroll
+            for (int i = 0; i < COPIES; ++i) {
+              copy16(sub + place[i % PLACES] + i * 512, k + i * 512);
+              copy16(sub + TILE + place[i % PLACES] + i * 512, v + i * 512);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < COPIES; ++i) {
+              const bool valid = mask >> (i * STEP + copy_row) & 1u;
+              copy16(sub + place[i % PLACES] + i * 512, valid ? k + i * 512 : p.k, valid ? 16 : 0);
+              copy16(sub + TILE + place[i % PLACES] + i * 512, valid ? v + i * 512 : p.v, valid ? 16 : 0);
+            }
           }
         } else {
+          const int* entries = p.table + in.of->slot * p.table_stride;
 #pragma unroll
           for (int i = 0; i < COPIES; ++i) {
-            const bool valid = mask >> (i * STEP + copy_row) & 1u;
-            copy16(to + place[i % PLACES] + i * 512, valid ? k + i * 512 : p.k, valid ? 16 : 0);
-            copy16(to + TILE + place[i % PLACES] + i * 512, valid ? v + i * 512 : p.v, valid ? 16 : 0);
+            const int r = i * STEP + copy_row, token = t0 + u * 16 + r;
+            bool valid = r < live;
+            const long long page = valid ? __ldg(entries + (token >> p.page_shift)) : 0;
+            if (page < 0 || page >= p.pages) { report(p); valid = false; }
+            // one bit per row, from the first lane of each row
+            const uint32_t votes = __ballot_sync(0xffffffffu, valid);
+#pragma unroll
+            for (int j = 0; j < STEP; ++j) mask |= (votes >> (j * LANES) & 1u) << (i * STEP + j);
+            const long long row = (long long)(token & in_page) * ROW + copy_chunk * 16;
+            copy16(sub + place[i % PLACES] + i * 512, valid ? p.k + page * p.k_page + kv * p.k_head + row : p.k, valid ? 16 : 0);
+            copy16(sub + TILE + place[i % PLACES] + i * 512, valid ? p.v + page * p.v_page + kv * p.v_head + row : p.v, valid ? 16 : 0);
           }
         }
-      } else {
-        const int* entries = p.table + in.of->slot * p.table_stride;
-#pragma unroll
-        for (int i = 0; i < COPIES; ++i) {
-          const int r = i * STEP + copy_row, token = t0 + r;
-          bool valid = r < live;
-          const long long page = valid ? __ldg(entries + (token >> p.page_shift)) : 0;
-          if (page < 0 || page >= p.pages) { report(p); valid = false; }
-          // one bit per row, from the first lane of each row
-          const uint32_t votes = __ballot_sync(0xffffffffu, valid);
-#pragma unroll
-          for (int j = 0; j < STEP; ++j) mask |= (votes >> (j * LANES) & 1u) << (i * STEP + j);
-          const long long row = (long long)(token & in_page) * ROW + copy_chunk * 16;
-          copy16(to + place[i % PLACES] + i * 512, valid ? p.k + page * p.k_page + kv * p.k_head + row : p.k, valid ? 16 : 0);
-          copy16(to + TILE + place[i % PLACES] + i * 512, valid ? p.v + page * p.v_page + kv * p.v_head + row : p.v, valid ? 16 : 0);
-        }
+        all_mask |= mask << (u * 16);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -274,7 +290,7 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
         if (in.tile == 0) warm();
       }
     }
-    return mask;
+    return all_mask;
   };
   if (in.left > 0) warm();
   uint32_t stage = ring, mask = fetch(ring), next_mask = fetch(ring + 2 * TILE);
@@ -342,34 +358,37 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
       asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
       __syncwarp();
       if (mask) {
-        float s[2][4];
+        float s[TOK / 8][4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        for (int n = 0; n < TOK / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) {
           if (FP8) {
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
+            for (int n = 0; n < TOK / 8; ++n) {
               uint32_t w;
               asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(((stage + fp8_lane) ^ (j * 16)) + n * 8 * ROW) : "memory");
               mma<true>(s[n], q[j], e4m3_to_f16(w & 0xffffu), e4m3_to_f16(w >> 16));
             }
           } else {
-            uint32_t b[4];
-            ldsm4(b, (stage + key_lane) ^ (j * 32));
-            mma<false>(s[0], q[j], b[0], b[1]);
-            mma<false>(s[1], q[j], b[2], b[3]);
+#pragma unroll
+            for (int u = 0; u < SUBS; ++u) {
+              uint32_t b[4];
+              ldsm4(b, ((stage + key_lane) ^ (j * 32)) + u * SUB);
+              mma<false>(s[u * 2], q[j], b[0], b[1]);
+              mma<false>(s[u * 2 + 1], q[j], b[2], b[3]);
+            }
           }
         }
         // scores in base 2; row g in elements 0 and 1, row g + 8 in 2 and 3; tokens 8 n + 2 t and the next
         float top[2] = {m[0], m[1]};
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < TOK / 8; ++n)
 #pragma unroll
           for (int i = 0; i < 2 * HALVES; ++i) s[n][i] *= score_scale[i >> 1];
-        if (mask != 0xffffu) {
+        if (mask != ALL) {
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+          for (int n = 0; n < TOK / 8; ++n)
 #pragma unroll
             for (int i = 0; i < 2 * HALVES; ++i)
               if (!(mask >> (n * 8 + t * 2 + (i & 1)) & 1u)) s[n][i] = -INFINITY;
@@ -377,7 +396,8 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
         bool higher = false;
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
-          top[h] = fmaxf(fmaxf(top[h], fmaxf(s[0][2 * h], s[0][2 * h + 1])), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+#pragma unroll
+          for (int n = 0; n < TOK / 8; ++n) top[h] = fmaxf(top[h], fmaxf(s[n][2 * h], s[n][2 * h + 1]));
           top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
           top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
           higher = higher || top[h] > m[h];
@@ -392,38 +412,41 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
             for (int n = 0; n < D / 8; ++n) { o[n][2 * h] *= a; o[n][2 * h + 1] *= a; }
           }
         }
-        uint32_t hi[4] = {}, lo[4] = {};                  // probabilities as an A fragment: rows g, g + 8; tokens 2 t, 2 t + 8
+        const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int h = i & 1;
-          if (h < HALVES) {
-            const float ref = m[h] == -INFINITY ? 0.f : m[h];
-            const float x = exp2_fast(s[i >> 1][h * 2] - ref), y = exp2_fast(s[i >> 1][h * 2 + 1] - ref);
-            l[h] += x + y;
-            if (FP8) {
-              hi[i] = pack_f16(x, y);
-            } else {
-              hi[i] = pack_bf16(x, y);
-              lo[i] = pack_bf16(x - tw::bf16_bits_to_float(hi[i] & 0xffffu), y - tw::bf16_bits_to_float(hi[i] >> 16));
+        for (int u = 0; u < SUBS; ++u) {
+          uint32_t hi[4] = {}, lo[4] = {};                // probabilities as an A fragment: rows g, g + 8; tokens 2 t, 2 t + 8
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int h = i & 1, n = u * 2 + (i >> 1);
+            if (h < HALVES) {
+              const float x = exp2_fast(s[n][h * 2] - ref[h]), y = exp2_fast(s[n][h * 2 + 1] - ref[h]);
+              l[h] += x + y;
+              if (FP8) {
+                hi[i] = pack_f16(x, y);
+              } else {
+                hi[i] = pack_bf16(x, y);
+                lo[i] = pack_bf16(x - tw::bf16_bits_to_float(hi[i] & 0xffffu), y - tw::bf16_bits_to_float(hi[i] >> 16));
+              }
             }
           }
-        }
 #pragma unroll
-        for (int c = 0; c < CHUNKS / 2; ++c) {
-          uint32_t b[4];
-          ldsm4_trans(b, (stage + TILE + value_lane) ^ (c * 32));
-          if (FP8) {
+          for (int c = 0; c < CHUNKS / 2; ++c) {
+            uint32_t b[4];
+            ldsm4_trans(b, ((stage + TILE + value_lane) ^ (c * 32)) + u * SUB);
+            if (FP8) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {                 // a chunk's 16 channels: the even ones and the odd ones
-              const uint32_t x = b[2 * h], y = b[2 * h + 1];
-              mma<true>(o[c * 4 + h * 2], hi, e4m3_to_f16(__byte_perm(x, 0, 0x4420)), e4m3_to_f16(__byte_perm(y, 0, 0x4420)));
-              mma<true>(o[c * 4 + h * 2 + 1], hi, e4m3_to_f16(__byte_perm(x, 0, 0x4431)), e4m3_to_f16(__byte_perm(y, 0, 0x4431)));
+              for (int h = 0; h < 2; ++h) {               // a chunk's 16 channels: the even ones and the odd ones
+                const uint32_t x = b[2 * h], y = b[2 * h + 1];
+                mma<true>(o[c * 4 + h * 2], hi, e4m3_to_f16(__byte_perm(x, 0, 0x4420)), e4m3_to_f16(__byte_perm(y, 0, 0x4420)));
+                mma<true>(o[c * 4 + h * 2 + 1], hi, e4m3_to_f16(__byte_perm(x, 0, 0x4431)), e4m3_to_f16(__byte_perm(y, 0, 0x4431)));
+              }
+            } else {
+              mma<false>(o[c * 2], hi, b[0], b[1]);
+              mma<false>(o[c * 2], lo, b[0], b[1]);
+              mma<false>(o[c * 2 + 1], hi, b[2], b[3]);
+              mma<false>(o[c * 2 + 1], lo, b[2], b[3]);
             }
-          } else {
-            mma<false>(o[c * 2], hi, b[0], b[1]);
-            mma<false>(o[c * 2], lo, b[0], b[1]);
-            mma<false>(o[c * 2 + 1], hi, b[2], b[3]);
-            mma<false>(o[c * 2 + 1], lo, b[2], b[3]);
           }
         }
       }
@@ -556,14 +579,14 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const __grid_c
 // CTAs that run beside each other, for units of which there are at most `most`.
 int grid_of(long long most) { const long long fit = 148 * 3; return (int)(most < 1 ? 1 : most < fit ? most : fit); }
 int grid_of(int batch, int hq, int hk, long long tokens) {
-  const long long tiles = (hq / hk + 15) / 16;
-  return grid_of((long long)batch * hk * tiles * ((tokens + UNIT - 1) / UNIT + 1));
+  const long long tiles = (hq / hk + 15) / 16, unit = WARPS * tile_tokens(256);          // the shortest unit
+  return grid_of((long long)batch * hk * tiles * ((tokens + unit - 1) / unit + 1));
 }
 int part_rows(int hq, int hk) { return hq / hk < 16 ? hq / hk : 16; }
 
 template <int D, bool FP8, bool WIDE>
 int launch(const Params& p, cudaStream_t stream) {
-  constexpr int SMEM = WARPS * 2 * 2 * 16 * D * (FP8 ? 1 : 2) + 256;
+  constexpr int ROW = D * (FP8 ? 1 : 2), SMEM = WARPS * 2 * 2 * tile_tokens(ROW) * ROW + 256;
   static std::atomic<bool> configured[64];            // the shared-memory opt-in is a per-device attribute of the function
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) { (void)cudaGetLastError(); return TW_ERR_LAUNCH; }
@@ -608,7 +631,7 @@ extern "C" int tw_paged_attention(const TwPagedAttentionArgs* a, void* stream) {
   const long long tokens = (long long)a->max_pages * a->page;
   const int tiles = (a->hq / a->hk + 15) / 16, heads = a->hk * tiles;
   if (a->page > (1 << 20) || tokens > (1LL << 30) || (long long)a->batch * heads > (1 << 30) ||
-      (long long)a->batch * heads * ((tokens + UNIT - 1) / UNIT + 1) > (1LL << 31) - 1)
+      (long long)a->batch * heads * (tokens / (WARPS * tile_tokens(256)) + 2) > (1LL << 31) - 1)
     return TW_ERR_TOO_LARGE;
   const int bytes = a->fp8 ? 1 : 2;
   if (misaligned(a->q, 4) || (a->q_stride_batch | a->q_stride_head) & 1 || misaligned(a->k_pages, 16) || misaligned(a->v_pages, 16) ||
