@@ -54,6 +54,23 @@ def _device(device):
     return _same_device if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
+# Scratch per stream: calls on one stream run one after the other. A call that is being captured gets scratch of its own graph's, so
+# that two graphs captured on one stream may be replayed side by side; only the newest capture's is held here, older ones live as
+# long as their graph's pool. 'zeroed' is 8 bytes that kernels leave zeroed (the graph zeroes its own on every replay), 'paged'
+# needs no initialisation and grows as wanted.
+_stream_scratch = {}
+
+
+def _scratch(device, stream, kind='zeroed', nbytes=8):
+    capture = _lib.load().tw_capture_id(stream)
+    key = (device, stream, kind, capture != 0)
+    held = _stream_scratch.get(key)
+    if held is None or held[0] != capture or held[1].numel() < nbytes:
+        make = torch.zeros if kind == 'zeroed' else torch.empty
+        held = _stream_scratch[key] = (capture, make(nbytes, device=device, dtype=torch.uint8))
+    return held[1]
+
+
 @dataclass
 class Packed:
     """Quantized activation: the reference's (codes, scales, factor, mp) tuple plus the atom-layout
@@ -385,13 +402,13 @@ def paged_attention(q, k_pages, v_pages, table, lengths, *, slots=None, scale=No
     lse = torch.empty((batch, hq), device=dev, dtype=torch.float32) if return_lse else None
     lib = _lib.load()
     with _device(dev):
-        # scratch of the call's own: calls on several streams, and captured ones, do not share it
-        scratch = torch.empty(_scratch_bytes('tw_paged_attention_workspace', batch, hq, hk, dim, width * page), device=dev, dtype=torch.uint8)
+        stream = _stream(dev)
+        scratch = _scratch(dev, stream, 'paged', _scratch_bytes('tw_paged_attention_workspace', batch, hq, hk, dim, width * page))
         args = _lib.PagedAttentionArgs(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table.data_ptr(), lengths.data_ptr(), None if slots is None else slots.data_ptr(),
             _ptr(k_scale), _ptr(v_scale), out.data_ptr(), None if lse is None else lse.data_ptr(), scratch.data_ptr(), _cache_status(dev), qs[0], qs[1],
             ks[0], ks[1], vs[0], vs[1], table_stride, dim ** -.5 if scale is None else scale, batch, sequences, hq, hk, dim, page, pages, width, fp8)
-        _lib.check(lib.tw_paged_attention(ctypes.byref(args), _stream(dev)))
+        _lib.check(lib.tw_paged_attention(ctypes.byref(args), stream))
     return (out, lse) if return_lse else out
 
 
@@ -450,8 +467,9 @@ def cache_append_(k, v, k_pages, v_pages, table, lengths, refs, *, slots=None, c
         vs = v.stride()
     call = _lib.AppendArgs(k.data_ptr(), v.data_ptr(), _ptr(slots), _ptr(cu), _ptr(k_scale), _ptr(v_scale), ks[0], ks[1], vs[0], vs[1], batch, rows)
     with _device(dev):
-        scratch = torch.empty(_scratch_bytes('tw_cache_append_workspace', batch, rows), device=dev, dtype=torch.uint8)
-        _lib.check(_lib.load().tw_cache_append(ctypes.byref(args), ctypes.byref(call), scratch.data_ptr(), _stream(dev)))
+        stream = _stream(dev)
+        scratch = _scratch(dev, stream, 'paged', _scratch_bytes('tw_cache_append_workspace', batch, rows))
+        _lib.check(_lib.load().tw_cache_append(ctypes.byref(args), ctypes.byref(call), scratch.data_ptr(), stream))
 
 
 def cache_fork_(k_pages, v_pages, table, lengths, refs, parents, children):
@@ -467,8 +485,9 @@ def cache_fork_(k_pages, v_pages, table, lengths, refs, parents, children):
     if not count:
         return
     with _device(dev):
-        scratch = torch.empty(_scratch_bytes('tw_cache_fork_workspace', count), device=dev, dtype=torch.uint8)
-        _lib.check(_lib.load().tw_cache_fork(ctypes.byref(args), parents.data_ptr(), children.data_ptr(), count, scratch.data_ptr(), _stream(dev)))
+        stream = _stream(dev)
+        scratch = _scratch(dev, stream, 'paged', _scratch_bytes('tw_cache_fork_workspace', count))
+        _lib.check(_lib.load().tw_cache_fork(ctypes.byref(args), parents.data_ptr(), children.data_ptr(), count, scratch.data_ptr(), stream))
 
 
 def cache_free_(table, lengths, refs, slots, page_size):
@@ -487,8 +506,9 @@ def cache_compact_(k_pages, v_pages, table, lengths, refs):
     args, dev, *_ = _cache(k_pages, v_pages, table, lengths, refs)
     live = torch.empty((), device=dev, dtype=torch.int32)
     with _device(dev):
-        scratch = torch.empty(_scratch_bytes('tw_cache_compact_workspace', refs.numel()), device=dev, dtype=torch.uint8)
-        _lib.check(_lib.load().tw_cache_compact(ctypes.byref(args), live.data_ptr(), scratch.data_ptr(), _stream(dev)))
+        stream = _stream(dev)
+        scratch = _scratch(dev, stream, 'paged', _scratch_bytes('tw_cache_compact_workspace', refs.numel()))
+        _lib.check(_lib.load().tw_cache_compact(ctypes.byref(args), live.data_ptr(), scratch.data_ptr(), stream))
     return live
 
 
@@ -620,21 +640,6 @@ def rope_heads(x, cos, sin, *, norm=False, eps=1e-6):
                                          _ptr(sin), cos.shape[0], int(cos.dtype == torch.bfloat16), int(norm), float(eps),
                                          _stream(x.device)))
     return y
-
-
-# Scratch that a kernel leaves zeroed, one per stream: calls on one stream run one after the other. A call that is being
-# captured gets one of its own graph (zeroed by the graph on every replay), so that two graphs captured on one stream may
-# be replayed side by side; only the newest capture's is held here, older ones live as long as their graph's pool.
-_stream_scratch = {}
-
-
-def _scratch(device, stream):
-    capture = _lib.load().tw_capture_id(stream)
-    key = (device, stream, capture != 0)
-    held = _stream_scratch.get(key)
-    if held is None or held[0] != capture:
-        held = _stream_scratch[key] = (capture, torch.zeros(8, device=device, dtype=torch.uint8))
-    return held[1]
 
 
 def _overlap(a, b):
