@@ -44,7 +44,7 @@ struct Params {
   const uint8_t *wr, *wrs;
   const int *off, *wi, *wloc;
   void* out;
-  int rows, n, k, kb, nb, groups, ksplit, slots, entries, shared, dense, out_f32;
+  int rows, n, k, kb, nb, groups, ksplit, k_share, k_more, n_share, n_more, slots, entries, shared, dense, out_f32;
 };
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) {
@@ -101,9 +101,10 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_kernel(const __grid_constan
   __shared__ float unscale[32];
   __shared__ int counts[MAX_ROUNDS];               // bank blocks of a round
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int rank = p.ksplit > 1 ? (int)cluster_rank() : 0, group = blockIdx.x / p.ksplit;
-  const int kb0 = p.kb * rank / p.ksplit, nkb = p.kb * (rank + 1) / p.ksplit - kb0, max_kb = (p.kb + p.ksplit - 1) / p.ksplit;
-  const int nb0 = (int)((long long)p.nb * group / p.groups), rounds = (int)((long long)p.nb * (group + 1) / p.groups) - nb0;
+  const int rank = p.ksplit > 1 ? (int)cluster_rank() : 0, group = p.ksplit > 1 ? (blockIdx.x - rank) / p.ksplit : blockIdx.x;
+  // even shares, the first ones one larger: of K by rank, of the N128 blocks by cluster
+  const int kb0 = rank * p.k_share + min(rank, p.k_more), nkb = p.k_share + (rank < p.k_more), max_kb = p.k_share + (p.k_more > 0);
+  const int nb0 = group * p.n_share + min(group, p.n_more), rounds = p.n_share + (group < p.n_more);
   const int pitch = x_pitch(max_kb);
   uint8_t* ring = dynamic + warp * 2 * QUAD;                                                     // [WARPS][2][QUAD]
   uint8_t* xs = dynamic + WARPS * 2 * QUAD;                                                      // [rows][pitch]
@@ -113,8 +114,10 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_kernel(const __grid_constan
   if (p.ksplit > 1) cluster_arrive();              // waited for before the first store to a peer: it has to be running
   // this CTA's part of x on its way to shared memory while the weights' first blocks are fetched
   const int chunks = nkb * 16, items = p.rows * chunks;                           // of 8 values; 16 lanes have chunks of one row
+  const float per_chunk = 1.f / (float)chunks;
+  auto row_of = [&](int i) { return (int)(((float)i + .5f) * per_chunk); };       // i / chunks: both below 2^17, half a unit from any whole number
   for (int i = threadIdx.x; i < items; i += THREADS) {
-    const int r = i / chunks, c = i - r * chunks, kk = kb0 * 128 + c * 8;
+    const int r = row_of(i), c = i - r * chunks, kk = kb0 * 128 + c * 8;
     uint8_t* to = xs + r * pitch + x_chunk(c);
     if (kk < p.k) copy16(tw::smem_u32(to), p.x + r * p.x_stride + kk);
     else *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);                  // k % 32 == 0; zeros behind it
@@ -230,12 +233,12 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_kernel(const __grid_constan
   };
   open(in);
   if (in.w0 > 0) point();
-  fetch(0);
 
-  // ---- x d, rounded to bf16, in the order the lanes read it; then scaled f16 in place ------------------------------
+  // x d, rounded to bf16, in the order the lanes read it; then scaled f16 in place
+  auto stage_x = [&]() {
   asm volatile("cp.async.wait_group 1;" ::: "memory");         // a thread's own chunks: nobody else reads them before the barrier
   for (int i = threadIdx.x; i < items; i += THREADS) {
-    const int r = i / chunks, c = i - r * chunks, kk = kb0 * 128 + c * 8;
+    const int r = row_of(i), c = i - r * chunks, kk = kb0 * 128 + c * 8;
     uint4* to = reinterpret_cast<uint4*>(xs + r * pitch + x_chunk(c));
     const uint4 v = *to;
     uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -262,10 +265,9 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_kernel(const __grid_constan
     for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mates, top, o));
     if ((lane & 15) == 0 && top) atomicMax(&peak[r], top);
   }
-  fetch(1);
   __syncthreads();
   for (int i = threadIdx.x; i < items; i += THREADS) {
-    const int r = i / chunks, c = i - r * chunks;
+    const int r = row_of(i), c = i - r * chunks;
     // 2^shift brings the largest value to [2^14, 2^15); an all-zero row stays, and 2^shift stays a normal number
     const int shift = peak[r] ? min(14 - ((int)(peak[r] >> 23) - 127), 126) : 0;
     const float up = __uint_as_float((unsigned)(127 + shift) << 23);
@@ -281,6 +283,7 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_kernel(const __grid_constan
     *to = make_uint4(w[0], w[1], w[2], w[3]);
   }
   __syncthreads();
+  };
 
   // ---- products --------------------------------------------------------------------------------------------------
   const float factor = __ldg(p.factor);
@@ -331,36 +334,31 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_kernel(const __grid_constan
   };
   Cursor at{0, 0, 0, 0};
   open(at);
-  int slot = 0;
-  while (at.round < rounds) {
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
-    __syncwarp();
-    const uint8_t* codes = ring + slot * QUAD + lane * 16;
-    const int n = width(at);
-    const uint8_t *low = ring + slot * QUAD + 4096 + t * 2 + g * SCALE_PITCH, *high = low + 8 * SCALE_PITCH;
-    if (!BANK || at.at < at.w0) {
-      if (scale_pitch % 8) {             // where a row's scales begin within their first aligned word
+  // One copy of everything: the first two passes only fetch (and stage x between), the others multiply what was fetched two passes
+  // before. Code that runs once costs its way from L2, some 7 cycles an instruction.
+  for (int pass = 0; rounds > at.round; ++pass) {
+    const int slot = pass & 1;
+    int n = 0;
+    if (pass >= 2) {
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      __syncwarp();
+      n = width(at);
+      const uint8_t* codes = ring + slot * QUAD + lane * 16;
+      const uint8_t *low = ring + slot * QUAD + 4096 + t * 2 + g * SCALE_PITCH, *high = low + 8 * SCALE_PITCH;
+      const bool base = !BANK || at.at < at.w0;
+      if (base && scale_pitch % 8) {     // where a row's scales begin within their first aligned word
         const int row = (nb0 + at.round) * 128 + warp * 16 + g;
         low += (min(row, p.n - 1) * (uint32_t)scale_pitch) & 7;
         high += (min(row + 8, p.n - 1) * (uint32_t)scale_pitch) & 7;
       }
-      if (n == 4) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) multiply(codes + j * 1024, low + j * 8, high + j * 8, at.at + j);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 3; ++j)
-          if (j < n) multiply(codes + j * 1024, low + j * 8, high + j * 8, at.at + j);
-      }
-    } else {
       const int2* entry = list + (size_t)at.round * max_kb + at.at - at.w0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j < n) multiply(codes + j * 1024, low + j * 8, high + j * 8, entry[j].x);
+#pragma unroll 1
+      for (int j = 0; j < n; ++j, codes += 1024, low += 8, high += 8) multiply(codes, low, high, base ? at.at + j : entry[j].x);
+      __syncwarp();
     }
-    __syncwarp();
     fetch(slot);
-    slot ^= 1;
+    if (pass == 0) stage_x();
+    if (pass < 2) continue;
     at.at += n;
     if (at.at >= at.w0 + at.bank) {
       if (p.ksplit > 1) {                // the barrier of the round before; at first, the one that says that all ranks run
@@ -460,6 +458,8 @@ int launch(Params p, cudaStream_t stream) {
   }
   if (!best) return TW_ERR_TOO_LARGE;
   p.ksplit = best;
+  p.k_share = p.kb / best; p.k_more = p.kb % best;
+  p.n_share = p.nb / p.groups; p.n_more = p.nb % p.groups;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(p.groups * p.ksplit);
   config.blockDim = dim3(THREADS);
