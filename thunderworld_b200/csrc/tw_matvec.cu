@@ -4,7 +4,7 @@
 // W is code * group scale, W0 plus the W1 tiles of the bank. A code has 2 significant bits and a scale 4, so their product is
 // exact in f16 (2^-10 ... 2688), and the tensor cores multiply f16 exactly into 32-bit sums: m16n8k16 with 16 weight rows as A and
 // up to 8 rows of x as B. x is bf16, whose exponents f16 does not have: every CTA scales its part of a row by a power of two
-// that brings the largest finite value to [2^14, 2^15). That is exact but for values 2^29 below the largest, whose last
+// that brings the largest value to [2^14, 2^15). That is exact but for values 2^29 below the largest, whose last
 // bits, 2^-39 of the largest, are rounded away, far below the 2^-24 of the sums; the sums are scaled back.
 //
 // What bounds it is the read of the weights, 9/16 byte each, once. A lane loads 16 bytes of codes (32 of k) of two rows and the two
@@ -253,12 +253,12 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_kernel(const __grid_constan
       }
       *to = make_uint4(w[0], w[1], w[2], w[3]);
     }
+    // The largest size, infinity among them: a row that holds one is infinite or NaN whatever becomes of its other values. Bits of
+    // sizes order like integers; NaN, which would come out on top, counts as infinity.
     unsigned top = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const unsigned lo = (w[j] & 0x7fffu) << 16, hi = w[j] & 0x7fff0000u;
-      top = max(top, max(lo < 0x7f800000u ? lo : 0u, hi < 0x7f800000u ? hi : 0u));        // finite values only
-    }
+    for (int j = 0; j < 4; ++j) top = __vmaxu2(top, w[j] & 0x7fff7fffu);
+    top = min(max(top << 16, top & 0xffff0000u), 0x7f800000u);
     // 16 lanes hold chunks of one row, and enter together: items is a multiple of 16
     const unsigned mates = 0xffffu << (lane & 16);
 #pragma unroll
