@@ -24,6 +24,7 @@ namespace {
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 // Tokens of a warp's tile: 16 of 256-byte rows, 32 of shorter ones (the instructions beside the products are per tile).
 __host__ __device__ constexpr int tile_tokens(int row_bytes) { return row_bytes >= 256 ? 16 : 32; }
+constexpr int JOINING = 2;           // steps, of a unit each, that putting the warps' parts of a sequence together is counted as
 constexpr int JOIN_ROWS = 4;        // query rows that a CTA's warps put together at a time
 
 struct Params {
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
   // ---- this CTA's run: the lengths' prefix sums, in units -----------------------------------------------------------
   const int per = (p.batch + THREADS - 1) / THREADS, first_b = min(threadIdx.x * per, p.batch), last_b = min(first_b + per, p.batch);
   int mine = 0, slot_unused;
-  for (int b = first_b; b < last_b; ++b) { const int n = units_of(tokens_of(p, b, slot_unused)); mine += n ? n + 1 : 0; }
+  for (int b = first_b; b < last_b; ++b) { const int n = units_of(tokens_of(p, b, slot_unused)); mine += n ? n + JOINING : 0; }
   int before = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) { const int x = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += x; }
@@ -149,7 +150,7 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
   }
   const int step0 = shares.begin(blockIdx.x);
   for (int b = first_b, at = before * p.heads; b < last_b; ++b) {
-    const int n = units_of(tokens_of(p, b, slot_unused)), steps = n ? (n + 1) * p.heads : 0;
+    const int n = units_of(tokens_of(p, b, slot_unused)), steps = n ? (n + JOINING) * p.heads : 0;
     if (at <= step0 && step0 < at + steps) { start_b = b; start_offset = step0 - at; }
     at += steps;
   }
@@ -167,7 +168,7 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
   // to the next sequence, if the cursor is behind the units of its own
   auto settle = [&](Cursor& c) {
     if (c.tile < c.units) return;
-    --c.left;                                      // the joining step
+    c.left -= c.units + JOINING - c.tile;          // the joining steps, or what the run has of them
     c.tile = 0;
     int b = c.of->b, h = c.of->h + 1;
     __syncwarp();                                  // every lane has read what every lane writes now
@@ -193,10 +194,10 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
   in.left = shares.begin(blockIdx.x + 1) - step0;
   in.of = &sequences[0][warp];
   enter(in, start_b);
-  const int start_h = start_offset / (in.units + 1);
+  const int start_h = start_offset / (in.units + JOINING);
   in.of->h = start_h;
   in.of->kv = start_h / p.tiles;
-  in.tile = start_offset - start_h * (in.units + 1);
+  in.tile = start_offset - start_h * (in.units + JOINING);
   settle(in);                          // a run that begins with a joining step leaves it to the owner of the sequence's last unit
   Cursor at = in;
   at.of = &sequences[1][warp];
@@ -208,7 +209,7 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
     if (in.left > 0 && in.tile > 0) {
       const int begin = step0 - in.tile, previous = shares.begin((int)blockIdx.x - 1), row0 = (in.of->h - in.of->kv * p.tiles) * 16;
       if (previous <= begin)
-        border = make_int4(shares.owner(begin + in.units - 1) - (int)blockIdx.x + 2, ((int)blockIdx.x - 1) * 2 + (previous < begin - 1 ? 1 : 0),
+        border = make_int4(shares.owner(begin + in.units - 1) - (int)blockIdx.x + 2, ((int)blockIdx.x - 1) * 2 + (previous < begin - JOINING ? 1 : 0),
                            (in.of->b * p.hk + in.of->kv) * p.group + row0, min(p.group - row0, 16));
     }
     p.borders[blockIdx.x] = border;
@@ -580,7 +581,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) paged_join_kernel(const __grid_c
 int grid_of(long long most) { const long long fit = 148 * 3; return (int)(most < 1 ? 1 : most < fit ? most : fit); }
 int grid_of(int batch, int hq, int hk, long long tokens) {
   const long long tiles = (hq / hk + 15) / 16, unit = WARPS * tile_tokens(256);          // the shortest unit
-  return grid_of((long long)batch * hk * tiles * ((tokens + unit - 1) / unit + 1));
+  return grid_of((long long)batch * hk * tiles * ((tokens + unit - 1) / unit + JOINING));
 }
 int part_rows(int hq, int hk) { return hq / hk < 16 ? hq / hk : 16; }
 
@@ -631,7 +632,7 @@ extern "C" int tw_paged_attention(const TwPagedAttentionArgs* a, void* stream) {
   const long long tokens = (long long)a->max_pages * a->page;
   const int tiles = (a->hq / a->hk + 15) / 16, heads = a->hk * tiles;
   if (a->page > (1 << 20) || tokens > (1LL << 30) || (long long)a->batch * heads > (1 << 30) ||
-      (long long)a->batch * heads * (tokens / (WARPS * tile_tokens(256)) + 2) > (1LL << 31) - 1)
+      (long long)a->batch * heads * (tokens / (WARPS * tile_tokens(256)) + 1 + JOINING) > (1LL << 31) - 1)
     return TW_ERR_TOO_LARGE;
   const int bytes = a->fp8 ? 1 : 2;
   if (misaligned(a->q, 4) || (a->q_stride_batch | a->q_stride_head) & 1 || misaligned(a->k_pages, 16) || misaligned(a->v_pages, 16) ||
