@@ -169,16 +169,16 @@ def test_views_streams_graphs_and_out():
     from thunderworld_b200 import ops
     codes, scales = weights(500, 1024, 1)
     factor = torch.tensor(1e-3, device='cuda')
-    wide = rows_of(6, 3 * 1024, 2)
+    wide = rows_of(10, 4 * 1024, 2)
     x = wide[::2, 1024:2048]                                              # strided rows
     want = ops.fp4_matvec(x.contiguous(), codes, scales, factor)
     assert torch.equal(ops.fp4_matvec(x, codes, scales, factor), want)
-    odd = torch.zeros(3 * 1024 + 1, device='cuda', dtype=torch.bfloat16)[1:].view(3, 1024)   # rows that no 16-byte load can take
+    odd = torch.zeros((5, 1032), device='cuda', dtype=torch.bfloat16)[:, 1:1025]           # rows that no 16-byte load can take
     odd.copy_(x)
     assert torch.equal(ops.fp4_matvec(odd, codes, scales, factor), want)
     assert torch.equal(ops.fp4_matvec(x[1], codes, scales, factor), want[1])
-    assert torch.equal(ops.fp4_matvec(x.contiguous().view(1, 3, 1024), codes, scales, factor), want[None])
-    out = torch.full((3, 500), 7., device='cuda', dtype=torch.bfloat16)
+    assert torch.equal(ops.fp4_matvec(x.contiguous().view(1, 5, 1024), codes, scales, factor), want[None])
+    out = torch.full((5, 500), 7., device='cuda', dtype=torch.bfloat16)
     assert ops.fp4_matvec(x, codes, scales, factor, out=out) is out and torch.equal(out, want)
     a, b = torch.cuda.Stream(), torch.cuda.Stream()
     torch.cuda.synchronize()

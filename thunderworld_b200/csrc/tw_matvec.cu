@@ -19,10 +19,12 @@
 // its sums of 128 rows to their owners through distributed shared memory, one cluster barrier per 128 rows, waited for after the
 // next 128 rows' products. No workspace, no atomics on sums: the order is fixed.
 //
-// Measured (B200, weights from HBM, graph replay): 1 x 24576 x 6144 24.0 us (3.5 TB/s), 1 x 12288 x 4096 13.4 us, 8 x 16384 x 4096
-// 17.8 us, 1 x 2048 x 2048 5.2 us. Without the products the 24576 x 6144 case streams at 6.3 TB/s, without the copies it takes as
-// long as with both: the decoding's instructions (106 per block of 2048 weights, at half an issue per cycle and scheduler) are
-// what bounds the large cases, start (launch, x to f16: 4 us) and join the small ones.
+// Measured (B200, weights from HBM, graph replay; bytes of the weights over time): 1 x 24576 x 6144 23.3 us (3.7 TB/s), 1 x 12288 x
+// 4096 12.6 us, 8 x 16384 x 4096 17.2 us, 32 x 16384 x 4096 35.9 us, 5 x 6144 x 24576 with a quarter repaired 35.9 us (3.0 TB/s), 1 x
+// 2048 x 2048 4.7 us. What bounds it: of the 23 us of 24576 x 6144, some 7 are start (launch, instructions from L2, x to f16)
+// and join (cluster barriers, cold code); then the decoding and the stream of the weights hide each other in part only: without the
+// decoding, or without the copies, it takes 2 us and 1 us less, without both products and decoding 5 us. More warps (24 or 32
+// per SM), a third quad on the way, chains of products and x loaded ahead change nothing, the next block's codes ahead cost 1 us.
 #include <atomic>
 #include "tw_common.cuh"
 #include "../../include/twb200.h"
@@ -96,6 +98,7 @@ __device__ __forceinline__ int x_chunk(int c) { return (c >> 4) * 256 + (c & 3) 
 
 template <int MT, bool BANK>     // MT: groups of 8 x rows
 __global__ void __launch_bounds__(THREADS, 2) matvec_kernel(const __grid_constant__ Params p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");       // launched while the kernel before it drains; nothing is read until that is through
   extern __shared__ __align__(16) uint8_t dynamic[];
   __shared__ unsigned peak[32];
   __shared__ float unscale[32];
@@ -112,16 +115,26 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_kernel(const __grid_constan
   int2* list = reinterpret_cast<int2*>(landing + 2 * sum_floats(p.rows, p.ksplit));              // [rounds][max_kb], only with a bank
 
   if (p.ksplit > 1) cluster_arrive();              // waited for before the first store to a peer: it has to be running
-  // this CTA's part of x on its way to shared memory while the weights' first blocks are fetched
-  const int chunks = nkb * 16, items = p.rows * chunks;                           // of 8 values; 16 lanes have chunks of one row
-  const float per_chunk = 1.f / (float)chunks;
-  auto row_of = [&](int i) { return (int)(((float)i + .5f) * per_chunk); };       // i / chunks: both below 2^17, half a unit from any whole number
-  for (int i = threadIdx.x; i < items; i += THREADS) {
-    const int r = row_of(i), c = i - r * chunks, kk = kb0 * 128 + c * 8;
-    uint8_t* to = xs + r * pitch + x_chunk(c);
-    if (kk < p.k) copy16(tw::smem_u32(to), p.x + r * p.x_stride + kk);
-    else *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);                  // k % 32 == 0; zeros behind it
-  }
+  // This CTA's part of x on its way to shared memory while the weights' first blocks are fetched. Half a warp takes a K128 block of
+  // a row at a time, 8 values a lane, and an even share of them that lie one behind the other, so that rows change seldom.
+  const int units = p.rows * nkb, half = threadIdx.x >> 4, chunk = threadIdx.x & 15;
+  const int unit0 = half * units / (THREADS / 16), unit_count = (half + 1) * units / (THREADS / 16) - unit0;
+  const int first_row = unit0 / nkb, first_kb = unit0 - first_row * nkb;
+  auto each_unit = [&](auto&& body) {              // (row, block, last of this share in its row)
+    int r = first_row, b = first_kb;
+#pragma unroll 1
+    for (int u = unit_count; u > 0; --u) {
+      const bool last = u == 1 || b + 1 == nkb;
+      body(r, b, last);
+      if (++b == nkb) { b = 0; ++r; }
+    }
+  };
+  auto x_at = [&](int r, int b) { return reinterpret_cast<uint4*>(xs + r * pitch + b * 256 + x_chunk(chunk)); };
+  each_unit([&](int r, int b, bool) {
+    const int kk = (kb0 + b) * 128 + chunk * 8;
+    if (kk < p.k) copy16(tw::smem_u32(x_at(r, b)), p.x + r * p.x_stride + kk);
+    else *x_at(r, b) = make_uint4(0, 0, 0, 0);                                    // k % 32 == 0; zeros behind it
+  });
   asm volatile("cp.async.commit_group;" ::: "memory");
   if (threadIdx.x < 32) peak[threadIdx.x] = 0;
   if (BANK) {
@@ -236,53 +249,61 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_kernel(const __grid_constan
 
   // x d, rounded to bf16, in the order the lanes read it; then scaled f16 in place
   auto stage_x = [&]() {
-  asm volatile("cp.async.wait_group 1;" ::: "memory");         // a thread's own chunks: nobody else reads them before the barrier
-  for (int i = threadIdx.x; i < items; i += THREADS) {
-    const int r = row_of(i), c = i - r * chunks, kk = kb0 * 128 + c * 8;
-    uint4* to = reinterpret_cast<uint4*>(xs + r * pitch + x_chunk(c));
-    const uint4 v = *to;
-    uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    if (p.prescale && kk < p.k) {
-      const float4 d0 = __ldg(reinterpret_cast<const float4*>(p.prescale + kk)), d1 = __ldg(reinterpret_cast<const float4*>(p.prescale + kk) + 1);
-      const float d[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
+    float4 d0 = make_float4(1.f, 1.f, 1.f, 1.f), d1 = d0;
+    auto load_d = [&](int b) {
+      const int kk = (kb0 + b) * 128 + chunk * 8;
+      if (kk < p.k) { d0 = __ldg(reinterpret_cast<const float4*>(p.prescale + kk)); d1 = __ldg(reinterpret_cast<const float4*>(p.prescale + kk) + 1); }
+    };
+    if (p.prescale && unit_count > 0) load_d(first_kb);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");         // a thread's own chunks: nobody else reads them before the barrier
+    uint32_t top = 0;                    // sizes of two bf16 values
+    each_unit([&](int r, int b, bool last) {
+      uint4* to = x_at(r, b);
+      const uint4 v = *to;
+      uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      if (p.prescale) {
+        const float d[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const __nv_bfloat162 b2 = __floats2bfloat162_rn(__fmul_rn(tw::bf16_bits_to_float(w[j] & 0xffffu), d[2 * j]),
+                                                          __fmul_rn(tw::bf16_bits_to_float(w[j] >> 16), d[2 * j + 1]));
+          w[j] = *reinterpret_cast<const uint32_t*>(&b2);
+        }
+        *to = make_uint4(w[0], w[1], w[2], w[3]);
+        load_d(b + 1 == nkb ? 0 : b + 1);          // the next unit's
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = __vmaxu2(top, w[j] & 0x7fff7fffu);
+      if (last) {
+        // The largest size, infinity among them: a row that holds one is infinite or NaN whatever becomes of its other values. Bits
+        // of sizes order like integers; NaN, which would come out on top, counts as infinity.
+        const uint32_t most = min(max(top << 16, top & 0xffff0000u), 0x7f800000u);
+        if (most) atomicMax(&peak[r], most);
+        top = 0;
+      }
+    });
+    __syncthreads();
+    int known = -1;
+    float up = 0.f;
+    each_unit([&](int r, int b, bool) {
+      if (r != known) {
+        // 2^shift brings the largest value to [2^14, 2^15); an all-zero row stays, and 2^shift stays a normal number
+        const int shift = peak[r] ? min(14 - ((int)(peak[r] >> 23) - 127), 126) : 0;
+        up = __uint_as_float((unsigned)(127 + shift) << 23);
+        if (b == 0 && chunk == 0) unscale[r] = __uint_as_float((unsigned)(127 - shift) << 23);
+        known = r;
+      }
+      uint4* to = x_at(r, b);
+      const uint4 v = *to;
+      uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const __nv_bfloat162 b = __floats2bfloat162_rn(__fmul_rn(tw::bf16_bits_to_float(w[j] & 0xffffu), d[2 * j]),
-                                                       __fmul_rn(tw::bf16_bits_to_float(w[j] >> 16), d[2 * j + 1]));
-        w[j] = *reinterpret_cast<const uint32_t*>(&b);
+        const __half2 h = __floats2half2_rn(tw::bf16_bits_to_float(w[j] & 0xffffu) * up, tw::bf16_bits_to_float(w[j] >> 16) * up);
+        w[j] = *reinterpret_cast<const uint32_t*>(&h);
       }
       *to = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    // The largest size, infinity among them: a row that holds one is infinite or NaN whatever becomes of its other values. Bits of
-    // sizes order like integers; NaN, which would come out on top, counts as infinity.
-    unsigned top = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) top = __vmaxu2(top, w[j] & 0x7fff7fffu);
-    top = min(max(top << 16, top & 0xffff0000u), 0x7f800000u);
-    // 16 lanes hold chunks of one row, and enter together: items is a multiple of 16
-    const unsigned mates = 0xffffu << (lane & 16);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mates, top, o));
-    if ((lane & 15) == 0 && top) atomicMax(&peak[r], top);
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < items; i += THREADS) {
-    const int r = row_of(i), c = i - r * chunks;
-    // 2^shift brings the largest value to [2^14, 2^15); an all-zero row stays, and 2^shift stays a normal number
-    const int shift = peak[r] ? min(14 - ((int)(peak[r] >> 23) - 127), 126) : 0;
-    const float up = __uint_as_float((unsigned)(127 + shift) << 23);
-    if (c == 0) unscale[r] = __uint_as_float((unsigned)(127 - shift) << 23);
-    uint4* to = reinterpret_cast<uint4*>(xs + r * pitch + x_chunk(c));
-    const uint4 v = *to;
-    uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const __half2 h = __floats2half2_rn(tw::bf16_bits_to_float(w[j] & 0xffffu) * up, tw::bf16_bits_to_float(w[j] >> 16) * up);
-      w[j] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    *to = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-  __syncthreads();
+    });
+    __syncthreads();
   };
 
   // ---- products --------------------------------------------------------------------------------------------------
@@ -318,6 +339,7 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_kernel(const __grid_constan
   // A round's sums over this CTA's part of K are in `landing`, its owners' share of them from every rank; rank q adds its share,
   // elements (x row, weight row) q * share ..., in the order of the ranks.
   const int elements = p.rows * 128, share = (elements + p.ksplit - 1) / p.ksplit, floats = sum_floats(p.rows, p.ksplit);
+  const float per_share = 1.f / (float)share;
   auto join = [&](int done) {
     const float* from = landing + (done & 1) * floats;
     for (int j = threadIdx.x; j < share && rank * share + j < elements; j += THREADS) {
@@ -376,7 +398,7 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_kernel(const __grid_constan
           const int col = m * 8 + 2 * t + (h & 1), e = col * 128 + warp * 16 + g + (h >> 1) * 8;
           const float y = CHAINS == 1 ? acc[m][0][h] : acc[m][0][h] + acc[m][CHAINS - 1][h];
           if (col < p.rows) {
-            if (p.ksplit > 1) { const int owner = e / share; peer_store(mine + rank * share + e - owner * share, owner, y * unscale[col]); }
+            if (p.ksplit > 1) { const int owner = (int)(((float)e + .5f) * per_share); peer_store(mine + rank * share + e - owner * share, owner, y * unscale[col]); }
             else mine[e] = y * unscale[col];
           }
         }
@@ -465,12 +487,14 @@ int launch(Params p, cudaStream_t stream) {
   config.blockDim = dim3(THREADS);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
-  cudaLaunchAttribute cluster;
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = p.ksplit;
-  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-  config.attrs = &cluster;
-  config.numAttrs = best > 1 ? 1 : 0;
+  cudaLaunchAttribute attributes[2];
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = p.ksplit;
+  attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+  config.attrs = attributes;
+  config.numAttrs = best > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&config, kernel, p);
   if (e != cudaSuccess) (void)cudaGetLastError();
   return e == cudaSuccess ? TW_OK : TW_ERR_LAUNCH;
