@@ -123,6 +123,7 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
   __shared__ int sums[WARPS + 1], start_b, start_offset;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   auto units_of = [](int tokens) { return (tokens + UNIT - 1) / UNIT; };
+  if (threadIdx.x == 0) start_b = start_offset = 0;
 
   // ---- this CTA's run: the lengths' prefix sums, in units -----------------------------------------------------------
   const int per = (p.batch + THREADS - 1) / THREADS, first_b = min(threadIdx.x * per, p.batch), last_b = min(first_b + per, p.batch);
@@ -174,7 +175,8 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
     __syncwarp();                                  // every lane has read what every lane writes now
     if (h == p.heads) {
       h = 0;
-      if (c.left > 0) do enter(c, ++b); while (c.units == 0);
+      // (the bounds matter only if somebody changes the lengths meanwhile)
+      if (c.left > 0) do enter(c, b = min(b + 1, p.batch - 1)); while (c.units == 0 && b + 1 < p.batch);
     }
     c.of->h = h;
     c.of->kv = h / p.tiles;
@@ -194,7 +196,7 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
   in.left = shares.begin(blockIdx.x + 1) - step0;
   in.of = &sequences[0][warp];
   enter(in, start_b);
-  const int start_h = start_offset / (in.units + JOINING);
+  const int start_h = min(start_offset / (in.units + JOINING), p.heads - 1);       // below it, unless the lengths have changed
   in.of->h = start_h;
   in.of->kv = start_h / p.tiles;
   in.tile = start_offset - start_h * (in.units + JOINING);
@@ -209,7 +211,7 @@ __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __gri
     if (in.left > 0 && in.tile > 0) {
       const int begin = step0 - in.tile, previous = shares.begin((int)blockIdx.x - 1), row0 = (in.of->h - in.of->kv * p.tiles) * 16;
       if (previous <= begin)
-        border = make_int4(shares.owner(begin + in.units - 1) - (int)blockIdx.x + 2, ((int)blockIdx.x - 1) * 2 + (previous < begin - JOINING ? 1 : 0),
+        border = make_int4(min(shares.owner(begin + in.units - 1), p.grid - 1) - (int)blockIdx.x + 2, ((int)blockIdx.x - 1) * 2 + (previous < begin - JOINING ? 1 : 0),
                            (in.of->b * p.hk + in.of->kv) * p.group + row0, min(p.group - row0, 16));
     }
     p.borders[blockIdx.x] = border;
