@@ -309,6 +309,9 @@ def test_refusals():
                         (lambda: ops.cache_append_(x, x, *pools, c.table, c.lengths, c.refs[:3]), 'refs'), (lambda: ops.cache_append_(x, x, *pools, c.table.t(), c.lengths, c.refs), 'table'),
                         (lambda: ops.cache_append_(x, x, c.k_pages[:1].expand(6, 2, 4, 64), c.v_pages, *tables), 'expanded'),
                         (lambda: ops.cache_append_(x, x, *pools, c.table[:1].expand(12, -1), c.lengths, c.refs), 'overlap'),
+                        (lambda: ops.cache_append_(c.k_pages[0, :, :2].transpose(0, 1), x, *pools, *tables), 'lie in the pages'),
+                        (lambda: ops.cache_append_(x, c.k_pages[5, :, 2:].transpose(0, 1), *pools, *tables), 'lie in the pages'),
+                        (lambda: ops.cache_append_(x, x, c.k_pages, c.k_pages, *tables), 'same memory'), (lambda: ops.cache_compact_(c.k_pages, c.k_pages, *tables), 'same memory'),
                         (lambda: ops.cache_fork_(*pools, *tables, s, s[:1]), 'one child'), (lambda: ops.cache_fork_(*pools, *tables, s.float(), s), 'parents'),
                         (lambda: ops.cache_free_(*tables, s.long(), 4), 'slots'), (lambda: ops.cache_free_(*tables, s, 3), 'power of two'),
                         (lambda: ops.cache_compact_(*pools, c.table, c.lengths[:3], c.refs), 'lengths'),
@@ -324,6 +327,32 @@ def test_refusals():
     c.fork(s[:0], s[:0])
     c.free(s[:0])
     assert all(torch.equal(a, b) for a, b in zip(before, tables))
+
+
+@gpu
+def test_pools_of_one_buffer():
+    """Keys and values as the halves of one tensor are two pools, not one."""
+    from thunderworld_b200 import ops
+    both = torch.zeros(6, 2, 2, 4, 64, device='cuda', dtype=torch.bfloat16)
+    c = make(6, 4, 2, 64, False)
+    k, v = torch.randn(2, 3, 2, 64, device='cuda').bfloat16()
+    ops.cache_append_(k, v, both[:, 0], both[:, 1], c.table, c.lengths, c.refs, slots=i32([0]), cu=i32([0, 3]))
+    page = int(c.table[0, 0])
+    assert torch.equal(both[page, 0, :, :3], k.transpose(0, 1)) and torch.equal(both[page, 1, :, :3], v.transpose(0, 1))
+
+
+@gpu
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float8_e4m3fn])
+def test_a_new_cache_takes_no_more_than_its_pages(dtype):
+    from thunderworld_b200 import PagedCache
+    c = PagedCache(4096, 64, 8, 128, sequences=4, max_tokens=1024, dtype=dtype)
+    assert c.k_pages.shape == (4096, 8, 64, 128) and c.k_pages.dtype is dtype and not c.v_pages.float().any()
+    del c
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    c = PagedCache(4096, 64, 8, 128, sequences=4, max_tokens=1024, dtype=dtype)
+    pages = 2 * c.k_pages.numel() * c.k_pages.element_size()
+    assert torch.cuda.max_memory_allocated() - before < 1.01 * pages + 2 ** 20
 
 
 def test_refusals_without_a_gpu():

@@ -101,6 +101,18 @@ def test_bank(r, n, k, share, shared):
 
 
 @gpu
+def test_a_bank_without_an_entry_adds_nothing():
+    """A layer that selects no tile of a bank that others use."""
+    from thunderworld_b200 import ops
+    codes, scales = weights(256, 512, 5)
+    bank, _ = bank_of(256, 512, .5, 6, True)
+    none = torch.zeros(0, dtype=torch.int32, device='cuda')
+    x, factor = rows_of(3, 512, 7), torch.tensor(1e-3, device='cuda')
+    y = ops.fp4_matvec(x, codes, scales, factor, wr=bank['wr'], wrs=bank['wrs'], wi=none, wloc=none, off=torch.zeros_like(bank['off']), shared=True)
+    assert torch.equal(y, ops.fp4_matvec(x, codes, scales, factor))
+
+
+@gpu
 def test_bank_entries_that_lead_outside_are_left_out():
     from thunderworld_b200 import ops
     n, k = 256, 1024
@@ -251,7 +263,8 @@ def test_refusals():
                        (dict(factor=torch.tensor(1.)), 'share a CUDA device'), (dict(wr=codes.view(1, 128, 64)), 'wrs'),
                        (dict(wr=codes.view(1, 128, 64), wrs=scales.view(1, 128, 8)), 'wi'),
                        (dict(wr=codes.view(1, 128, 64), wrs=scales.view(1, 128, 8), wi=torch.zeros(1, dtype=torch.int32, device='cuda'),
-                             off=torch.zeros(3, dtype=torch.int32, device='cuda')), 'off')):
+                             off=torch.zeros(3, dtype=torch.int32, device='cuda')), 'off'), (dict(out=x), 'share memory'),
+                       (dict(x=(wide := rows_of(4, 256, 2))[:, :128], out=wide.view(8, 128)[:4]), 'share memory')):
         args = dict(x=x, codes=codes, scales=scales, factor=f) | bad
         with pytest.raises(ValueError, match=match):
             call(args.pop('x'), args.pop('codes'), args.pop('scales'), args.pop('factor'), **args)

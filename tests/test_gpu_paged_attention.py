@@ -265,7 +265,8 @@ def test_refusals():
                        (dict(lengths=i32(3)), 'lengths'), (dict(lengths=i32(2).long()), 'lengths'), (dict(lengths=i32(2).cpu()), 'lengths'),
                        (dict(slots=i32(3)), 'slots'), (dict(slots=i32(2).long()), 'slots'), (dict(table=i32(1, 5), lengths=i32(1)), 'slots'),
                        (dict(k_scale=torch.ones(2, device='cuda')), 'float8'), (dict(k_pages=f8, v_pages=f8, k_scale=torch.ones(3, device='cuda')), 'k_scale'),
-                       (dict(k_pages=f8, v_pages=f8, v_scale=torch.ones(2)), 'v_scale'), (dict(out=torch.zeros(2, 4, 64, device='cuda')), 'out must')):
+                       (dict(k_pages=f8, v_pages=f8, v_scale=torch.ones(2)), 'v_scale'), (dict(out=torch.zeros(2, 4, 64, device='cuda')), 'out must'),
+                       (dict(out=ok['q']), 'share memory')):
         with pytest.raises(ValueError, match=match):
             ops.paged_attention(**(ok | bad))
     with pytest.raises(RuntimeError, match='inference'):

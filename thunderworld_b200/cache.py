@@ -1,6 +1,7 @@
 """A paged key-value cache for a token at a time: the pool of pages, the tables that say whose they are, and the operators of
 `ops` on them. Everything that changes lives on the device (page tables, lengths, reference counts), nothing is read back, so that a
-step that appends, attends, forks or frees can be captured in a CUDA Graph after one call of each kind has run.
+step that appends, attends, forks or frees can be captured in a CUDA Graph after one call of each kind has run. Calls on one cache
+belong on one stream, or in an order that events give them.
 
 The reference keeps the keys and values of its autoregressive prefix per layer in contiguous tensors
 (thunderworld_fp4/cosmos/ar_cache.py:57-153); there is no paged cache in it.
@@ -24,7 +25,10 @@ class PagedCache:
         if min(pages, page_size, kv_heads, sequences, max_tokens) < 1:
             raise ValueError('pages, page_size, kv_heads, sequences and max_tokens must be positive')
         self.page_size = page_size
-        self.k_pages, self.v_pages = (torch.zeros((pages, kv_heads, page_size, head_dim), device=device, dtype=torch.bfloat16).to(dtype) for _ in range(2))
+        if dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+            raise ValueError('pages must be bfloat16 or float8_e4m3fn')
+        shape = pages, kv_heads, page_size, head_dim * dtype.itemsize
+        self.k_pages, self.v_pages = (torch.zeros(shape, device=device, dtype=torch.uint8).view(dtype) for _ in range(2))
         self.table = torch.full((sequences, ops.cdiv(max_tokens, page_size)), -1, device=device, dtype=torch.int32)
         self.lengths = torch.zeros(sequences, device=device, dtype=torch.int32)
         self.refs = torch.zeros(pages, device=device, dtype=torch.int32)

@@ -522,7 +522,7 @@ extern "C" int tw_matvec(const TwMatvecArgs* a, void* stream) {
   p.wr = a->wr; p.wrs = a->wrs; p.off = a->off; p.wi = a->wi; p.wloc = a->wloc; p.out = a->out;
   p.rows = a->rows; p.n = a->n; p.k = a->k; p.kb = (a->k + 127) / 128; p.nb = (a->n + 127) / 128;
   p.slots = a->slots; p.entries = a->entries; p.shared = a->shared; p.dense = a->dense; p.out_f32 = a->out_f32;
-  // 32 rows at a time, or what fits a cluster: 16 rows for a K above 13 k, 8 for a K above 28 k
+  // 32 rows at a time, or what fits a cluster of 8: 16 rows of a K above 14336, 8 with a bank and a K above 31744
   int most = 32;
   while (most > 8 && smem_bytes(most, p.kb, p.kb < 8 ? p.kb : 8, bank ? MAX_ROUNDS : 0) > MOST_SMEM) most /= 2;
   const int passes = (a->rows + most - 1) / most, step = (a->rows + passes - 1) / passes;

@@ -232,9 +232,9 @@ def fp4_matvec(x, codes, scales, factor, *, prescale=None, bias=None, wr=None, w
 
     y = factor * (bf16(x * prescale) @ W.T) + bias, W = codes [N, K/2] x E4M3 scales [N, K/16] plus the W1 tiles of a bank
     (wr [slots, 128, 64], wrs [slots, 128, 8]; wi, off, wloc, shared, dense as in fused_gemm), sums of 32 bits, one rounding.
-    factor: float32 scalar tensor; prescale float32 [K]; bias bf16 [N]; out_dtype bfloat16 or float32. Any N, K a multiple of
-    32 up to 32768; with a bank both multiples of 128. One launch (two for more rows of a K above 13 k than fit
-    an SM's shared memory)."""
+    factor: float32 scalar tensor; prescale float32 [K]; bias bf16 [N]; out_dtype bfloat16 or float32; out shares no memory with x. Any
+    N, K a multiple of 32 up to 32768; with a bank both multiples of 128. One launch; where the rows' part of K does not fit an SM's
+    shared memory (more than 16 rows of a K above 14336, with a bank more than 8 of a K above 31744) two to four, a share of the rows each."""
     if x.ndim < 1 or x.dtype is not torch.bfloat16 or not x.is_cuda:
         raise ValueError('expected CUDA BF16 rows [..., K]')
     if codes.ndim != 2 or codes.dtype is not torch.uint8 or not codes.is_contiguous():
@@ -260,7 +260,7 @@ def fp4_matvec(x, codes, scales, factor, *, prescale=None, bias=None, wr=None, w
         raise ValueError(f'at most {MATVEC_ROWS} rows; more go through the quantizer and fused_gemm')
     if torch.is_grad_enabled() and x.requires_grad:
         raise RuntimeError('fp4_matvec is inference-only; use torch.inference_mode()')
-    slots = 0 if wr is None else wr.shape[0]
+    slots = 0 if wr is None or (wi is not None and not dense and not wi.numel()) else wr.shape[0]     # a bank without an entry adds nothing
     if slots:
         if n % 128 or k % 128:
             raise ValueError('a W1 bank needs N and K to be multiples of 128')
@@ -288,6 +288,8 @@ def fp4_matvec(x, codes, scales, factor, *, prescale=None, bias=None, wr=None, w
         out = torch.empty(shape, device=dev, dtype=out_dtype)
     elif tuple(out.shape) != shape or out.dtype is not out_dtype or not out.is_contiguous() or out.device != dev:
         raise ValueError(f'out must be contiguous {out_dtype} {shape} on the device of x')
+    elif _meet(_span(out), _span(flat)):
+        raise ValueError('out must not share memory with x')
     args = _lib.MatvecArgs(flat.data_ptr(), flat.stride(0) if rows > 1 else k, _ptr(prescale), codes.data_ptr(), scales.data_ptr(),
                            factor.data_ptr(), _ptr(bias), _ptr(wr) if slots else None, _ptr(wrs) if slots else None, _ptr(wi),
                            _ptr(off), _ptr(wloc), out.data_ptr(), rows, n, k, slots, 0 if wi is None else wi.numel(),
@@ -330,6 +332,18 @@ def _check_pages(k_pages, v_pages):
     if not k_pages.is_cuda or v_pages.device != k_pages.device:
         raise ValueError('pages must be on one CUDA device')
     return pages, hk, page, dim, dtype is torch.float8_e4m3fn, ks, vs
+
+
+def _span(t):
+    """First and last address of a nonempty tensor's elements."""
+    first, last = t.data_ptr(), -1
+    for n, s in zip(t.shape, t.stride()):
+        last += (n - 1) * s
+    return first, first + (last + 2) * t.element_size() - 1
+
+
+def _meet(a, b):
+    return a[0] <= b[1] and b[0] <= a[1]
 
 
 def _check_int32(device, name, t):
@@ -399,6 +413,8 @@ def paged_attention(q, k_pages, v_pages, table, lengths, *, slots=None, scale=No
         out = torch.empty(shape, device=dev, dtype=torch.bfloat16)
     elif out.shape != shape or out.dtype is not torch.bfloat16 or not out.is_contiguous() or out.device != dev:
         raise ValueError(f'out must be contiguous BF16 {tuple(shape)} on the device of the pages')
+    elif _meet(_span(out), _span(q)):
+        raise ValueError('out must not share memory with q')
     lse = torch.empty((batch, hq), device=dev, dtype=torch.float32) if return_lse else None
     lib = _lib.load()
     with _device(dev):
@@ -419,6 +435,8 @@ def _cache(k_pages, v_pages, table, lengths, refs, page=None):
         if (pages > 1 and not (ks[0] and vs[0])) or (hk > 1 and not (ks[1] and vs[1])):
             raise ValueError('pages are written: they must not be expanded')
         dev, pointers = k_pages.device, (k_pages.data_ptr(), v_pages.data_ptr())
+        if pointers[0] == pointers[1]:
+            raise ValueError('pages are written: k_pages and v_pages must not be the same memory')
     else:
         dev, pages, hk, dim, fp8, ks, vs, pointers = refs.device, refs.numel(), 0, 0, False, (0, 0), (0, 0), (None, None)
         if type(page) is not int or page < 1 or page & (page - 1):
@@ -465,7 +483,16 @@ def cache_append_(k, v, k_pages, v_pages, table, lengths, refs, *, slots=None, c
     if vs[2] != 1 or vs[0] % 8 or vs[1] % 8 or v.data_ptr() % 16:
         v = v.clone(memory_format=torch.contiguous_format)
         vs = v.stride()
-    call = _lib.AppendArgs(k.data_ptr(), v.data_ptr(), _ptr(slots), _ptr(cu), _ptr(k_scale), _ptr(v_scale), ks[0], ks[1], vs[0], vs[1], batch, rows)
+    pages, _, page, _ = k_pages.shape
+    width = 1 if fp8 else 2
+    k_at, v_at, new_k, new_v = args.k_pages, args.v_pages, k.data_ptr(), v.data_ptr()
+    k_end = k_at + ((pages - 1) * args.k_stride_page + (hk - 1) * args.k_stride_head + page * dim) * width
+    v_end = v_at + ((pages - 1) * args.v_stride_page + (hk - 1) * args.v_stride_head + page * dim) * width
+    for at, (row, head, _) in ((new_k, ks), (new_v, vs)):
+        end = at + ((rows - 1) * row + (hk - 1) * head + dim) * 2
+        if (at < k_end and k_at < end) or (at < v_end and v_at < end):
+            raise ValueError('k and v must not lie in the pages')
+    call = _lib.AppendArgs(new_k, new_v, _ptr(slots), _ptr(cu), _ptr(k_scale), _ptr(v_scale), ks[0], ks[1], vs[0], vs[1], batch, rows)
     with _device(dev):
         stream = _stream(dev)
         scratch = _scratch(dev, stream, 'paged', _scratch_bytes('tw_cache_append_workspace', batch, rows))
@@ -474,8 +501,8 @@ def cache_append_(k, v, k_pages, v_pages, table, lengths, refs, *, slots=None, c
 
 def cache_fork_(k_pages, v_pages, table, lengths, refs, parents, children):
     """Slot children[i], which must be empty and may be named once, becomes a copy of slot parents[i] as it was before the call: full
-    pages are shared (refs counts their holders), the rows of a partly filled last page are copied to the lowest free page. int32 [n] each. A call that cannot be
-    done changes nothing and shows in device_status()."""
+    pages are shared (refs counts their holders), the rows of a partly filled last page are copied to the lowest free page. int32 [n]
+    each. A call that cannot be done changes nothing and shows in device_status()."""
     args, dev, *_ = _cache(k_pages, v_pages, table, lengths, refs)
     _check_int32(dev, 'parents', parents)
     _check_int32(dev, 'children', children)
