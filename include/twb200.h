@@ -135,7 +135,7 @@ int tw_fused_tile_n(int n);
  * tw_fused for a token at a time. x stays bf16 (no activation planes), sums are 32 bits wide, one rounding at the end.
  * W[n, k] = code * scale (scale per 16 k), plus the bank's tile where (n / 128, k / 128) has one; bank layout, CSR, shared and
  * dense as in TwRepairIO, every (n / 128, k / 128) at most once. Any n; k % 32 == 0, k <= 32768; with a bank n and k multiples of 128.
- * Entries of off / wi / wloc that lead outside wi, K or the bank are left out. */
+ * Entries of off / wi / wloc that lead outside wi, K or the bank are left out. out must not overlap x. */
 typedef struct TwMatvecArgs {
   const void* x;            /* bf16, row r at x + r * x_stride, 16-byte aligned rows */
   long long x_stride;       /* elements, a multiple of 8 */
@@ -203,7 +203,8 @@ int tw_attention(const TwAttentionArgs* args, void* stream);
  * sequence gives zeros and lse = -inf. What lies behind a sequence's end in its last page is not used, whatever it is.
  * Pages: [pages, hk, page, dim], rows contiguous, bf16 or (fp8) E4M3; page a power of two; dim 64 or 128; any hq / hk.
  * A slot, length or table entry that leads outside is left out (its tokens do not count) and reported in *status. Scratch needs no
- * initialisation; calls that may overlap need scratch of their own. Two launches. */
+ * initialisation; calls that may overlap need scratch of their own, and must not overlap a call that changes the cache.
+ * out must not overlap q. Two launches. */
 typedef struct TwPagedAttentionArgs {
   const void* q;                 /* bf16, q[b, h, :] at q + b * q_stride_batch + h * q_stride_head; even strides */
   const void *k_pages, *v_pages;
@@ -224,7 +225,8 @@ int tw_paged_attention(const TwPagedAttentionArgs* args, void* stream);
  * State on the device: table [sequences, max_pages] (page numbers, -1 behind a sequence's pages), lengths [sequences] (tokens), refs
  * [pages] (sequences that hold a page, 0: free). All calls are asynchronous and can be captured. append, fork and compact change
  * nothing when they cannot be done, and raise *status to "a page table entry, slot or length leads outside the cache" or "the
- * page pool or a sequence's table is full"; free leaves out what leads outside, and reports it. sequences <= 65536. */
+ * page pool or a sequence's table is full"; free leaves out what leads outside, and reports it. sequences <= 65536. The two pools
+ * share no memory, and the rows that append reads lie outside them. */
 typedef struct TwCache {
   void *k_pages, *v_pages;       /* [pages, hk, page, dim], rows contiguous, bf16 or (fp8) E4M3, 16-byte aligned heads */
   int32_t *table, *lengths, *refs;
@@ -243,8 +245,8 @@ typedef struct TwAppendArgs {
 } TwAppendArgs;
 size_t tw_cache_append_workspace(int batch, int rows);
 int tw_cache_append(const TwCache* cache, const TwAppendArgs* args, void* workspace, void* stream);
-/* children[i] (an empty slot, named once) becomes a copy of parents[i] as it was before the call: full pages are shared, the rows of a partly filled last page
- * are copied to the lowest free page. */
+/* children[i] (an empty slot, named once) becomes a copy of parents[i] as it was before the call: full pages are shared, the rows of
+ * a partly filled last page are copied to the lowest free page. */
 size_t tw_cache_fork_workspace(int count);
 int tw_cache_fork(const TwCache* cache, const int32_t* parents, const int32_t* children, int count, void* workspace, void* stream);
 /* Empties the slots: their pages lose a reference, their table entries become -1. Naming a slot twice is naming it once. */

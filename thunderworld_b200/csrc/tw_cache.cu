@@ -8,6 +8,8 @@
 // one pass over refs: block-wide prefix sums give every request its page, so the result does not depend on any order of execution),
 // then the copies by the whole device, which is what takes the time where there is much to copy (HBM-bound, 16 bytes a lane). A call whose
 // plan does not work out (an entry outside, a slot twice, a full pool) changes nothing and reports it in the status word.
+// Measured (B200): compact's copies of 91 MB of pages (64 tokens, 8 heads of 128, bf16) 27.1 us, 6.6 TB/s read and written; append and fork
+// of tens of sequences copy a microsecond or two: they are held by their two launches.
 #include "tw_common.cuh"
 #include "../../include/twb200.h"
 

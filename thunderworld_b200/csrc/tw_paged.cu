@@ -3,9 +3,10 @@
 // for G = hq / hk query heads per key head, head dimension 64 or 128, pages in bf16 or in E4M3 with a scale per key head.
 //
 // What bounds it is the read of the keys and values, once. The work is cut into units of 64 tokens of one (sequence, key head), 128
-// where a row is shorter than 256 bytes, in that order, and the units are shared evenly by the CTAs that run beside each other, whatever the lengths (which only the device
-// knows; putting the warps' parts of a sequence together costs about a unit and is counted as one): a CTA's run may begin and end inside a sequence, and what it has of such a one goes to the workspace, unnormalised, with
-// its maximum and sum; a second small launch joins these in their order. A call needs no zeroed state and no counter, so calls
+// where a row is shorter than 256 bytes, in that order, and the units are shared evenly by the CTAs that run beside each other,
+// whatever the lengths (which only the device knows; putting the warps' parts of a sequence together is counted as two more): a
+// CTA's run may begin and end inside a sequence, and what it has of such a one goes to the workspace, unnormalised, with its
+// maximum and sum; a second small launch joins these in their order. A call needs no zeroed state and no counter, so calls
 // on several streams, and captured ones, do not meet.
 // A warp takes 16 (32) of a unit's tokens: it copies their rows (two units ahead) to a ring of its own, multiplies q (the group's heads,
 // padded to 16 rows) by the keys, keeps its own running maximum and sum in 32 bits, base 2, and multiplies the probabilities
@@ -15,6 +16,13 @@
 // products are in f16, which holds E4M3 exactly, and q is scaled by a power of two per head to the range of f16.
 // Tokens behind a sequence's end, and those of a table entry outside the pool (reported in the status word), are masked
 // and read as zeros, whatever lies there.
+//
+// Measured (B200, pages from HBM, graph replay; both launches; 32 heads on 8 or 4, dim 128): 24 sequences of 0 ... 8192 tokens in pages of
+// 16 69.2 us (5.4 TB/s of keys and values); 48 of up to 16384 with E4M3 pages 69 us (4.1 TB/s); one of 100000 tokens 75.8 us
+// (5.4 TB/s); 32 of 4096 41.7 us (4.5 TB/s); one of 3840 tokens 15.1 us. The large bf16 cases are held by memory (12 warps per SM wait for it, long
+// scoreboard the first stall); with E4M3 pages the instructions per byte double (1.6 issued per cycle and SM); small calls by
+// their chain of start, lengths, table, pages, warps' join, second launch. Three times as many smaller runs, an earlier launch of
+// the join and branch hints changed nothing.
 #include <atomic>
 #include "tw_common.cuh"
 #include "../../include/twb200.h"
@@ -22,9 +30,12 @@
 namespace {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
-// Tokens of a warp's tile: 16 of 256-byte rows, 32 of shorter ones (the instructions beside the products are per tile).
+// Tokens of a warp's tile: 16 of 256-byte rows, 32 of shorter ones: the instructions beside the products are per tile (48 sequences of
+// E4M3 pages 82.4 us with 16, 77.3 us with 32), and 32 of 256 bytes would take the shared memory of a CTA.
 __host__ __device__ constexpr int tile_tokens(int row_bytes) { return row_bytes >= 256 ? 16 : 32; }
-constexpr int JOINING = 2;           // steps, of a unit each, that putting the warps' parts of a sequence together is counted as
+// Steps, of a unit each, that putting the warps' parts of a sequence together is counted as. 1, 2, 3: 24 ragged sequences 76.4, 70.3,
+// 68.8 us; 64 of 2000 tokens in pages of one token, where a unit takes longer, 23.7, 24.2, 26.5 us.
+constexpr int JOINING = 2;
 constexpr int JOIN_ROWS = 4;        // query rows that a CTA's warps put together at a time
 
 struct Params {
@@ -109,7 +120,8 @@ struct Cursor {
   Sequence* of;
 };
 
-// WIDE: more than 8 query rows per tile; else the lower half of the 16 rows is all there is, and nothing is computed for the rest.
+// WIDE: more than 8 query heads per key head; else the upper 8 of a tile's 16 rows do not exist, and nothing is computed for them
+// (maxima, exponentials and sums are half of a tile's arithmetic).
 template <int D, bool FP8, bool WIDE>
 __global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __grid_constant__ Params p) {
   constexpr int ROW = D * (FP8 ? 1 : 2), CHUNKS = ROW / 16, TOK = tile_tokens(ROW), SUBS = TOK / 16, UNIT = WARPS * TOK;
