@@ -19,7 +19,7 @@
 //
 // Measured (B200, pages from HBM, graph replay; both launches; 32 heads on 8 or 4, dim 128): 24 sequences of 0 ... 8192 tokens in pages of
 // 16 69.2 us (5.4 TB/s of keys and values); 48 of up to 16384 with E4M3 pages 69 us (4.1 TB/s); one of 100000 tokens 75.8 us
-// (5.4 TB/s); 32 of 4096 41.7 us (4.5 TB/s); one of 3840 tokens 15.1 us. The large bf16 cases are held by memory (12 warps per SM wait for it, long
+// (5.4 TB/s); 32 of 4096 41.7 us (4.5 TB/s); one of 3840 tokens 14.2 us. The large bf16 cases are held by memory (12 warps per SM wait for it, long
 // scoreboard the first stall); with E4M3 pages the instructions per byte double (1.6 issued per cycle and SM); small calls by
 // their chain of start, lengths, table, pages, warps' join, second launch. Three times as many smaller runs, an earlier launch of
 // the join and branch hints changed nothing.
@@ -30,6 +30,7 @@
 namespace {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
+constexpr int SMS = 148;
 // Tokens of a warp's tile: 16 of 256-byte rows, 32 of shorter ones: the instructions beside the products are per tile (48 sequences of
 // E4M3 pages 82.4 us with 16, 77.3 us with 32), and 32 of 256 bytes would take the shared memory of a CTA.
 __host__ __device__ constexpr int tile_tokens(int row_bytes) { return row_bytes >= 256 ? 16 : 32; }
@@ -105,9 +106,12 @@ __device__ __forceinline__ float weight_of(float m, float top) { return m == -IN
 template <int CHUNKS> __device__ __forceinline__ int swizzled(int c, int r) { return CHUNKS == 4 ? c ^ (r >> 1 & 3) : c ^ (r & 7); }
 
 // Shares of `all` steps: the first all % owners owners have a step more than the others.
+// An owner per SM before any has two steps, then no more owners than have two: a second CTA on an SM for one step, and its part to join,
+// cost more than they take off the others (1 x 3840 tokens, 8 key heads, 15.2 with an owner per step, 14.2 us; 1 x 30000, one key head of 64
+// channels, 17.0, 13.8; 1 x 16384, 32 heads on one, 29.0, 24.5; at least four steps: 14.5, 14.7, 26.2).
 struct Shares {
   int all, owners, per, more;
-  __device__ __forceinline__ Shares(int all_, int grid) : all(all_), owners(min(all_, grid)) { per = owners ? all / owners : 0; more = all - per * owners; }
+  __device__ __forceinline__ Shares(int all_, int grid) : all(all_), owners(min(max((all_ + 1) / 2, min(all_, SMS)), grid)) { per = owners ? all / owners : 0; more = all - per * owners; }
   __device__ __forceinline__ int begin(int c) const { return c * per + min(c, more); }
   __device__ __forceinline__ int owner(int u) const { return u < more * (per + 1) ? u / (per + 1) : more + (u - more * (per + 1)) / per; }
 };
@@ -591,7 +595,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const __gri
 }
 
 // CTAs that run beside each other, for units of which there are at most `most`.
-int grid_of(long long most) { const long long fit = 148 * 3; return (int)(most < 1 ? 1 : most < fit ? most : fit); }
+int grid_of(long long most) { const long long fit = SMS * 3; return (int)(most < 1 ? 1 : most < fit ? most : fit); }
 int grid_of(int batch, int hq, int hk, long long tokens) {
   const long long tiles = (hq / hk + 15) / 16, unit = WARPS * tile_tokens(256);          // the shortest unit
   return grid_of((long long)batch * hk * tiles * ((tokens + unit - 1) / unit + JOINING));
