@@ -20,7 +20,7 @@
 // next 128 rows' products. No workspace, no atomics on sums: the order is fixed.
 //
 // Measured (B200, weights from HBM, graph replay; bytes of the weights over time): 1 x 24576 x 6144 23.3 us (3.7 TB/s), 1 x 12288 x
-// 4096 12.6 us, 8 x 16384 x 4096 17.2 us, 32 x 16384 x 4096 35.9 us, 5 x 6144 x 24576 with a quarter repaired 35.9 us (3.0 TB/s), 1 x
+// 4096 12.6 us, 8 x 16384 x 4096 16.9 us, 32 x 16384 x 4096 36.1 us, 5 x 6144 x 24576 with a quarter repaired 35.9 us (3.0 TB/s), 1 x
 // 2048 x 2048 4.7 us. What bounds it: of the 23 us of 24576 x 6144, some 7 are start (launch, instructions from L2, x to f16)
 // and join (cluster barriers, cold code); then the decoding and the stream of the weights hide each other in part only: without the
 // decoding, or without the copies, it takes 2 us and 1 us less, without both products and decoding 5 us. More warps (24 or 32
@@ -460,8 +460,9 @@ int launch(Params p, cudaStream_t stream) {
     if (device < 64) configured[device].store(true, std::memory_order_relaxed);
   }
   // The cluster size that leaves a warp the fewest blocks: rounds of 128 rows times blocks per round, a round's barrier and
-  // sums counted as 2 MT blocks. More clusters than run beside each other would wait for the others; one CTA on an SM
-  // instead of two has half the warps to hide its latencies.
+  // sums counted as MT blocks, the staging of a block of 8 rows of x as one (8 x 16384 x 4096 17.3 us with the barrier as 2 MT, 16.9
+  // with MT; 32 x 16384 x 4096 42.4 us with 4 MT, 36.1 with MT). More clusters than run beside each other would wait for the others;
+  // one CTA on an SM instead of two has half the warps to hide its latencies.
   int best = 0, best_cost = 1 << 30;
   size_t smem = 0;
   for (int ksplit = 1; ksplit <= 8 && ksplit <= p.kb; ++ksplit) {
@@ -473,7 +474,7 @@ int launch(Params p, cudaStream_t stream) {
       const int rounds = (p.nb + groups - 1) / groups;
       const size_t need = smem_bytes(p.rows, p.kb, ksplit, BANK ? rounds : 0);
       if (need > (size_t)(per_sm == 2 ? PAIR_SMEM : MOST_SMEM)) continue;
-      const int cost = rounds * (kbs + 2 * MT) + p.rows * kbs / 8;
+      const int cost = 8 * rounds * (kbs + MT) + p.rows * kbs;
       if (cost < best_cost) { best = ksplit; best_cost = cost; p.groups = groups; smem = need; }
       break;
     }

@@ -111,7 +111,7 @@ template <int CHUNKS> __device__ __forceinline__ int swizzled(int c, int r) { re
 // channels, 17.0, 13.8; 1 x 16384, 32 heads on one, 29.0, 24.5; at least four steps: 14.5, 14.7, 26.2).
 struct Shares {
   int all, owners, per, more;
-  __device__ __forceinline__ Shares(int all_, int grid) : all(all_), owners(min(max((all_ + 1) / 2, min(all_, SMS)), grid)) { per = owners ? all / owners : 0; more = all - per * owners; }
+  __device__ __forceinline__ Shares(int all_, int grid) : all(all_), owners(min(max(all_ - all_ / 2, min(all_, SMS)), grid)) { per = owners ? all / owners : 0; more = all - per * owners; }
   __device__ __forceinline__ int begin(int c) const { return c * per + min(c, more); }
   __device__ __forceinline__ int owner(int u) const { return u < more * (per + 1) ? u / (per + 1) : more + (u - more * (per + 1)) / per; }
 };
