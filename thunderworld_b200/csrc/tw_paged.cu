@@ -31,6 +31,10 @@ namespace {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int SMS = 148;
+// CTAs per SM: three, so of at most 168 registers a thread; two where 16 query rows of 128 channels need more than that (up to 252;
+// 32 sequences of 8192 tokens, 32 heads on 2: 47.9 us with three, 38.4 with two; E4M3 39.8, 31.0). 16 rows of 64 channels fit
+// (64 sequences 34.9 us with three, 37.7 with two).
+__host__ __device__ constexpr int ctas_per_sm(int dim, bool wide) { return wide && dim == 128 ? 2 : 3; }
 // Tokens of a warp's tile: 16 of 256-byte rows, 32 of shorter ones: the instructions beside the products are per tile (48 sequences of
 // E4M3 pages 82.4 us with 16, 77.3 us with 32), and 32 of 256 bytes would take the shared memory of a CTA.
 __host__ __device__ constexpr int tile_tokens(int row_bytes) { return row_bytes >= 256 ? 16 : 32; }
@@ -107,8 +111,8 @@ template <int CHUNKS> __device__ __forceinline__ int swizzled(int c, int r) { re
 
 // Shares of `all` steps: the first all % owners owners have a step more than the others.
 // An owner per SM before any has two steps, then no more owners than have two: a second CTA on an SM for one step, and its part to join,
-// cost more than they take off the others (1 x 3840 tokens, 8 key heads, 15.2 with an owner per step, 14.2 us; 1 x 30000, one key head of 64
-// channels, 17.0, 13.8; 1 x 16384, 32 heads on one, 29.0, 24.5; at least four steps: 14.5, 14.7, 26.2).
+// cost more than they take off the others (1 x 3840 tokens, 8 key heads, 15.2 with an owner per step, 14.2 us; 1 x 30000, one key head
+// of 64 channels, 17.0, 13.8; 1 x 16384, 32 heads on one, 29.0, 24.5; at least four steps: 14.5, 14.7, 26.2).
 struct Shares {
   int all, owners, per, more;
   __device__ __forceinline__ Shares(int all_, int grid) : all(all_), owners(min(max(all_ - all_ / 2, min(all_, SMS)), grid)) { per = owners ? all / owners : 0; more = all - per * owners; }
@@ -127,7 +131,7 @@ struct Cursor {
 // WIDE: more than 8 query heads per key head; else the upper 8 of a tile's 16 rows do not exist, and nothing is computed for them
 // (maxima, exponentials and sums are half of a tile's arithmetic).
 template <int D, bool FP8, bool WIDE>
-__global__ void __launch_bounds__(THREADS, 3) paged_attention_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(THREADS, ctas_per_sm(D, WIDE)) paged_attention_kernel(const __grid_constant__ Params p) {
   constexpr int ROW = D * (FP8 ? 1 : 2), CHUNKS = ROW / 16, TOK = tile_tokens(ROW), SUBS = TOK / 16, UNIT = WARPS * TOK;
   constexpr int SUB = 16 * ROW, TILE = SUBS * SUB;         // bytes of 16 tokens' rows, of a tile's
   constexpr uint32_t ALL = TOK == 32 ? 0xffffffffu : 0xffffu;
@@ -594,11 +598,11 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const __gri
   if (p.lse && lane == 0) p.lse[head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945f;
 }
 
-// CTAs that run beside each other, for units of which there are at most `most`.
-int grid_of(long long most) { const long long fit = SMS * 3; return (int)(most < 1 ? 1 : most < fit ? most : fit); }
-int grid_of(int batch, int hq, int hk, long long tokens) {
+// CTAs that run beside each other, or as many as there may be units.
+int grid_of(int batch, int hq, int hk, int dim, long long tokens) {
   const long long tiles = (hq / hk + 15) / 16, unit = WARPS * tile_tokens(256);          // the shortest unit
-  return grid_of((long long)batch * hk * tiles * ((tokens + unit - 1) / unit + JOINING));
+  const long long most = (long long)batch * hk * tiles * ((tokens + unit - 1) / unit + JOINING), fit = SMS * ctas_per_sm(dim, hq / hk > 8);
+  return (int)(most < 1 ? 1 : most < fit ? most : fit);
 }
 int part_rows(int hq, int hk) { return hq / hk < 16 ? hq / hk : 16; }
 
@@ -638,7 +642,7 @@ bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_
 
 extern "C" size_t tw_paged_attention_workspace(int batch, int hq, int hk, int dim, long long tokens) {
   if (batch <= 0 || hk <= 0 || hq <= 0 || hq % hk || dim <= 0 || tokens < 0) return 0;
-  return (size_t)grid_of(batch, hq, hk, tokens) * (16 + 2 * part_rows(hq, hk) * (dim + 2) * 4);
+  return (size_t)grid_of(batch, hq, hk, dim, tokens) * (16 + 2 * part_rows(hq, hk) * (dim + 2) * 4);
 }
 
 extern "C" int tw_paged_attention(const TwPagedAttentionArgs* a, void* stream) {
@@ -666,7 +670,7 @@ extern "C" int tw_paged_attention(const TwPagedAttentionArgs* a, void* stream) {
   p.out = static_cast<__nv_bfloat16*>(a->out); p.lse = a->lse; p.status = a->status;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.batch = a->batch; p.sequences = a->sequences; p.hk = a->hk; p.group = a->hq / a->hk; p.tiles = tiles; p.heads = heads;
-  p.pages = a->pages; p.max_pages = a->max_pages; p.rows = part_rows(a->hq, a->hk); p.grid = grid_of(a->batch, a->hq, a->hk, tokens);
+  p.pages = a->pages; p.max_pages = a->max_pages; p.rows = part_rows(a->hq, a->hk); p.grid = grid_of(a->batch, a->hq, a->hk, a->dim, tokens);
   while ((1 << p.page_shift) < a->page) ++p.page_shift;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   p.borders = reinterpret_cast<int4*>(ws);
