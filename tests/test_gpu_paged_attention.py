@@ -106,6 +106,15 @@ def test_many_sequences(fp8):
 
 
 @gpu
+@pytest.mark.parametrize('hq,hk,dim', [(16, 1, 128), (16, 1, 64), (8, 1, 128), (24, 2, 128), (4, 1, 128)])
+@pytest.mark.parametrize('count', [2, 23, 37, 64, 101, 150])
+def test_runs_that_begin_and_end_anywhere(hq, hk, dim, count):
+    """Sequences of a few units, so that the CTAs' shares begin inside them, behind them and between two, and hold one, several or none."""
+    lens = [int(n) for n in torch.randint(0, 400, (count,), generator=torch.Generator().manual_seed(count))]
+    run(lens, hq, hk, dim, 16, count % 2 == 1, seed=count)
+
+
+@gpu
 @pytest.mark.parametrize('fp8', [False, True])
 def test_sharp_scores_and_scale(fp8):
     """Scores of hundreds, so that one token has all the weight, and a negative scale."""

@@ -4,7 +4,7 @@
 //
 // What bounds it is the read of the keys and values, once. The work is cut into units of 64 tokens of one (sequence, key head), 128
 // where a row is shorter than 256 bytes, in that order, and the units are shared evenly by the CTAs that run beside each other,
-// whatever the lengths (which only the device knows; putting the warps' parts of a sequence together is counted as two more): a
+// whatever the lengths (which only the device knows; putting the warps' parts of a sequence together is counted as a few more): a
 // CTA's run may begin and end inside a sequence, and what it has of such a one goes to the workspace, unnormalised, with its
 // maximum and sum; a second small launch joins these in their order. A call needs no zeroed state and no counter, so calls
 // on several streams, and captured ones, do not meet.
@@ -17,12 +17,12 @@
 // Tokens behind a sequence's end, and those of a table entry outside the pool (reported in the status word), are masked
 // and read as zeros, whatever lies there.
 //
-// Measured (B200, pages from HBM, graph replay; both launches; 32 heads on 8 or 4, dim 128): 24 sequences of 0 ... 8192 tokens in pages of
-// 16 69.2 us (5.4 TB/s of keys and values); 48 of up to 16384 with E4M3 pages 69 us (4.1 TB/s); one of 100000 tokens 75.8 us
-// (5.4 TB/s); 32 of 4096 41.7 us (4.5 TB/s); one of 3840 tokens 14.2 us. The large bf16 cases are held by memory (12 warps per SM wait for it, long
-// scoreboard the first stall); with E4M3 pages the instructions per byte double (1.6 issued per cycle and SM); small calls by
-// their chain of start, lengths, table, pages, warps' join, second launch. Three times as many smaller runs, an earlier launch of
-// the join and branch hints changed nothing.
+// Measured (B200, pages from HBM, graph replay; both launches; 32 heads on 8 or 4, dim 128): 24 sequences of 0 ... 8192 tokens in pages
+// of 16 69.2 us (5.4 TB/s of keys and values); 48 of up to 16384 with E4M3 pages 67 us (4.2 TB/s); one of 100000 tokens 76 us
+// (5.4 TB/s); 32 of 4096 41.1 us (4.5 TB/s); one of 3840 tokens 13.9 us; 32 of up to 8192 with 32 heads on 2 30.3 us (3.1 TB/s). The
+// large bf16 cases are held by memory (12 warps per SM wait for it, long scoreboard the first stall); with E4M3 pages the instructions
+// per byte double (1.6 issued per cycle and SM); small calls by their chain of start, lengths, table, pages, warps' join, second
+// launch. Three times as many smaller runs, an earlier launch of the join and branch hints changed nothing.
 #include <atomic>
 #include "tw_common.cuh"
 #include "../../include/twb200.h"
@@ -38,10 +38,12 @@ __host__ __device__ constexpr int ctas_per_sm(int dim, bool wide) { return wide 
 // Tokens of a warp's tile: 16 of 256-byte rows, 32 of shorter ones: the instructions beside the products are per tile (48 sequences of
 // E4M3 pages 82.4 us with 16, 77.3 us with 32), and 32 of 256 bytes would take the shared memory of a CTA.
 __host__ __device__ constexpr int tile_tokens(int row_bytes) { return row_bytes >= 256 ? 16 : 32; }
-// Steps, of a unit each, that putting the warps' parts of a sequence together is counted as. 1, 2, 3: 24 ragged sequences 76.4, 70.3,
-// 68.8 us; 64 of 2000 tokens in pages of one token, where a unit takes longer, 23.7, 24.2, 26.5 us.
-constexpr int JOINING = 2;
 constexpr int JOIN_ROWS = 4;        // query rows that a CTA's warps put together at a time
+// Steps, of a unit each, that putting the warps' parts of a sequence together is counted as: the more rows and channels, the more. 1, 2,
+// 3, 6 steps: 24 ragged sequences, 4 rows per key head 75.3, 69.0, 69.8, 70.1 us; 48 E4M3 ones of 8 rows 79.1, 69.1, 67.0, 69.4; 32 of up
+// to 8192 tokens and 16 rows 39.9, 38.5, 37.9, 30.2, with 64 channels (64 of them) 38.7, 35.6, 33.7, 34.2.
+constexpr int MOST_JOINING = 6;
+inline int joining_of(int rows, int dim) { return rows <= JOIN_ROWS ? 2 : rows <= 2 * JOIN_ROWS || dim == 64 ? 3 : MOST_JOINING; }
 
 struct Params {
   const __nv_bfloat16* q; long long q_batch, q_head;
@@ -54,7 +56,7 @@ struct Params {
   float *part_o, *part_ml;          // [grid][2][rows][dim], [grid][2][rows][2]
   int* status;
   float scale_log2;
-  int batch, sequences, hk, group, tiles, heads, page_shift, pages, max_pages, rows, grid;   // tiles of 16 query rows per key head; heads = hk * tiles
+  int batch, sequences, hk, group, tiles, heads, page_shift, pages, max_pages, rows, joining, grid;   // tiles of 16 query rows per key head; heads = hk * tiles
 };
 
 __device__ __forceinline__ void report(const Params& p) { if (p.status) atomicMax(p.status, (int)TW_ERR_PAGE); }
@@ -148,7 +150,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, WIDE)) paged_attention
   // ---- this CTA's run: the lengths' prefix sums, in units -----------------------------------------------------------
   const int per = (p.batch + THREADS - 1) / THREADS, first_b = min(threadIdx.x * per, p.batch), last_b = min(first_b + per, p.batch);
   int mine = 0, slot_unused;
-  for (int b = first_b; b < last_b; ++b) { const int n = units_of(tokens_of(p, b, slot_unused)); mine += n ? n + JOINING : 0; }
+  for (int b = first_b; b < last_b; ++b) { const int n = units_of(tokens_of(p, b, slot_unused)); mine += n ? n + p.joining : 0; }
   int before = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) { const int x = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += x; }
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, WIDE)) paged_attention
   }
   const int step0 = shares.begin(blockIdx.x);
   for (int b = first_b, at = before * p.heads; b < last_b; ++b) {
-    const int n = units_of(tokens_of(p, b, slot_unused)), steps = n ? (n + JOINING) * p.heads : 0;
+    const int n = units_of(tokens_of(p, b, slot_unused)), steps = n ? (n + p.joining) * p.heads : 0;
     if (at <= step0 && step0 < at + steps) { start_b = b; start_offset = step0 - at; }
     at += steps;
   }
@@ -189,7 +191,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, WIDE)) paged_attention
   // to the next sequence, if the cursor is behind the units of its own
   auto settle = [&](Cursor& c) {
     if (c.tile < c.units) return;
-    c.left -= c.units + JOINING - c.tile;          // the joining steps, or what the run has of them
+    c.left -= c.units + p.joining - c.tile;          // the joining steps, or what the run has of them
     c.tile = 0;
     int b = c.of->b, h = c.of->h + 1;
     __syncwarp();                                  // every lane has read what every lane writes now
@@ -216,10 +218,10 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, WIDE)) paged_attention
   in.left = shares.begin(blockIdx.x + 1) - step0;
   in.of = &sequences[0][warp];
   enter(in, start_b);
-  const int start_h = min(start_offset / (in.units + JOINING), p.heads - 1);       // below it, unless the lengths have changed
+  const int start_h = min(start_offset / (in.units + p.joining), p.heads - 1);       // below it, unless the lengths have changed
   in.of->h = start_h;
   in.of->kv = start_h / p.tiles;
-  in.tile = start_offset - start_h * (in.units + JOINING);
+  in.tile = start_offset - start_h * (in.units + p.joining);
   settle(in);                          // a run that begins with a joining step leaves it to the owner of the sequence's last unit
   Cursor at = in;
   at.of = &sequences[1][warp];
@@ -231,7 +233,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, WIDE)) paged_attention
     if (in.left > 0 && in.tile > 0) {
       const int begin = step0 - in.tile, previous = shares.begin((int)blockIdx.x - 1), row0 = (in.of->h - in.of->kv * p.tiles) * 16;
       if (previous <= begin)
-        border = make_int4(min(shares.owner(begin + in.units - 1), p.grid - 1) - (int)blockIdx.x + 2, ((int)blockIdx.x - 1) * 2 + (previous < begin - JOINING ? 1 : 0),
+        border = make_int4(min(shares.owner(begin + in.units - 1), p.grid - 1) - (int)blockIdx.x + 2, ((int)blockIdx.x - 1) * 2 + (previous < begin - p.joining ? 1 : 0),
                            (in.of->b * p.hk + in.of->kv) * p.group + row0, min(p.group - row0, 16));
     }
     p.borders[blockIdx.x] = border;
@@ -598,13 +600,13 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const __gri
   if (p.lse && lane == 0) p.lse[head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945f;
 }
 
+int part_rows(int hq, int hk) { return hq / hk < 16 ? hq / hk : 16; }
 // CTAs that run beside each other, or as many as there may be units.
 int grid_of(int batch, int hq, int hk, int dim, long long tokens) {
   const long long tiles = (hq / hk + 15) / 16, unit = WARPS * tile_tokens(256);          // the shortest unit
-  const long long most = (long long)batch * hk * tiles * ((tokens + unit - 1) / unit + JOINING), fit = SMS * ctas_per_sm(dim, hq / hk > 8);
+  const long long most = (long long)batch * hk * tiles * ((tokens + unit - 1) / unit + joining_of(part_rows(hq, hk), dim)), fit = SMS * ctas_per_sm(dim, hq / hk > 8);
   return (int)(most < 1 ? 1 : most < fit ? most : fit);
 }
-int part_rows(int hq, int hk) { return hq / hk < 16 ? hq / hk : 16; }
 
 template <int D, bool FP8, bool WIDE>
 int launch(const Params& p, cudaStream_t stream) {
@@ -653,7 +655,7 @@ extern "C" int tw_paged_attention(const TwPagedAttentionArgs* a, void* stream) {
   const long long tokens = (long long)a->max_pages * a->page;
   const int tiles = (a->hq / a->hk + 15) / 16, heads = a->hk * tiles;
   if (a->page > (1 << 20) || tokens > (1LL << 30) || (long long)a->batch * heads > (1 << 30) ||
-      (long long)a->batch * heads * (tokens / (WARPS * tile_tokens(256)) + 1 + JOINING) > (1LL << 31) - 1)
+      (long long)a->batch * heads * (tokens / (WARPS * tile_tokens(256)) + 1 + MOST_JOINING) > (1LL << 31) - 1)
     return TW_ERR_TOO_LARGE;
   const int bytes = a->fp8 ? 1 : 2;
   if (misaligned(a->q, 4) || (a->q_stride_batch | a->q_stride_head) & 1 || misaligned(a->k_pages, 16) || misaligned(a->v_pages, 16) ||
@@ -670,7 +672,8 @@ extern "C" int tw_paged_attention(const TwPagedAttentionArgs* a, void* stream) {
   p.out = static_cast<__nv_bfloat16*>(a->out); p.lse = a->lse; p.status = a->status;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.batch = a->batch; p.sequences = a->sequences; p.hk = a->hk; p.group = a->hq / a->hk; p.tiles = tiles; p.heads = heads;
-  p.pages = a->pages; p.max_pages = a->max_pages; p.rows = part_rows(a->hq, a->hk); p.grid = grid_of(a->batch, a->hq, a->hk, a->dim, tokens);
+  p.pages = a->pages; p.max_pages = a->max_pages; p.rows = part_rows(a->hq, a->hk); p.joining = joining_of(p.rows, a->dim);
+  p.grid = grid_of(a->batch, a->hq, a->hk, a->dim, tokens);
   while ((1 << p.page_shift) < a->page) ++p.page_shift;
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
   p.borders = reinterpret_cast<int4*>(ws);
