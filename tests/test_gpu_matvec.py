@@ -211,6 +211,45 @@ def test_views_streams_graphs_and_out():
 
 
 @gpu
+def test_a_captured_chain_over_two_streams():
+    """A call waits for what comes before it, whatever that is: a call on another stream, a copy, a fill, a call on its own stream."""
+    from thunderworld_b200 import ops
+    k = 1024
+    (c0, s0), (c1, s1) = weights(k, k, 11), weights(k, k, 12)
+    factor = torch.tensor(2e-3, device='cuda')
+    x = rows_of(2, k, 3)
+    side = torch.cuda.Stream()
+
+    def chain(x):
+        a, b = torch.empty(2, k, device='cuda', dtype=torch.bfloat16), torch.empty(2, k, device='cuda', dtype=torch.bfloat16)
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            ops.fp4_matvec(x[0], c0, s0, factor, out=a[0])
+        ops.fp4_matvec(x[1], c1, s1, factor, out=a[1])
+        main.wait_stream(side)
+        y = ops.fp4_matvec(a, c0, s0, factor)              # behind two calls
+        b.copy_(y)
+        z = ops.fp4_matvec(b, c1, s1, factor)              # behind a copy
+        b.zero_()
+        b[1] = z[0]
+        return y, z, ops.fp4_matvec(b, c0, s0, factor), ops.fp4_matvec(ops.fp4_matvec(z, c0, s0, factor), c1, s1, factor)
+    want = [t.clone() for t in chain(x)]
+    torch.cuda.synchronize()
+    held = torch.zeros_like(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain(held)
+    held.copy_(x)
+    for _ in range(20):
+        for t in got:
+            t.fill_(float('nan'))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
 def test_offsets_past_32_bits():
     """Codes of more than 4 GiB: rows at the end are read where they lie."""
     from thunderworld_b200 import ops
