@@ -299,3 +299,16 @@ def test_refusals_without_a_gpu():
     size = lib.tw_paged_attention_workspace
     assert size(0, 4, 2, 128, 64) == 0 and size(1, 3, 2, 128, 64) == 0 and size(1, 4, 2, 128, 0) > 0
     assert size(4, 8, 2, 128, 10 ** 6) <= 148 * 3 * (2 * 4 * 130 * 4 + 16)
+
+
+@gpu
+@pytest.mark.parametrize('fp8', [False, True])
+@pytest.mark.parametrize('hq,hk', [(4, 1), (16, 1), (6, 3)])
+def test_spans_of_empty_sequences(hq, hk, fp8):
+    """Between two sequences with tokens lie up to 200 without: a warp's cursor passes them and goes on in the right one."""
+    g = torch.Generator().manual_seed(hq)
+    lens = []
+    for span in (0, 200, 1, 33, 0, 128, 64, 7, 199, 3):
+        lens += [0] * span + [int(torch.randint(1, 500, (1,), generator=g))]
+    run(lens + [0] * 90, hq, hk, 64, 16, fp8, seed=hk)
+    run(lens + [0] * 90, hq, hk, 128, 4, fp8, seed=hk + 1)

@@ -180,28 +180,28 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, WIDE)) paged_attention
   __syncthreads();
 
   __shared__ Sequence sequences[2][WARPS];
-  auto enter = [&](Cursor& c, int b) {
-    int slot;
-    const int tokens = tokens_of(p, b, slot);
-    c.of->b = b;
-    c.of->slot = slot;
-    c.of->tokens = tokens;
-    c.units = units_of(tokens);
-  };
-  // to the next sequence, if the cursor is behind the units of its own
+  // To the next sequence, if the cursor is behind the units of its own. Every lane finds it in registers and writes what it found once,
+  // the same as the others: between two warp barriers, so that no lane reads what another has yet to write, or writes what another reads.
   auto settle = [&](Cursor& c) {
     if (c.tile < c.units) return;
     c.left -= c.units + p.joining - c.tile;          // the joining steps, or what the run has of them
     c.tile = 0;
-    int b = c.of->b, h = c.of->h + 1;
-    __syncwarp();                                  // every lane has read what every lane writes now
-    if (h == p.heads) {
-      h = 0;
+    int b = c.of->b, h = c.of->h + 1, slot = 0, tokens = 0;
+    const bool enters = h == p.heads && c.left > 0;
+    if (h == p.heads) h = 0;
+    if (enters) {
       // (the bounds matter only if somebody changes the lengths meanwhile)
-      if (c.left > 0) do enter(c, b = min(b + 1, p.batch - 1)); while (c.units == 0 && b + 1 < p.batch);
+      do c.units = units_of(tokens = tokens_of(p, b = min(b + 1, p.batch - 1), slot)); while (c.units == 0 && b + 1 < p.batch);
+    }
+    __syncwarp();
+    if (enters) {
+      c.of->b = b;
+      c.of->slot = slot;
+      c.of->tokens = tokens;
     }
     c.of->h = h;
     c.of->kv = h / p.tiles;
+    __syncwarp();
   };
   auto advance = [&](Cursor& c) { --c.left; ++c.tile; settle(c); };
 
@@ -217,15 +217,18 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, WIDE)) paged_attention
   Cursor in;
   in.left = shares.begin(blockIdx.x + 1) - step0;
   in.of = &sequences[0][warp];
-  enter(in, start_b);
+  int start_slot;
+  const int start_tokens = tokens_of(p, start_b, start_slot);
+  in.units = units_of(start_tokens);
   const int start_h = min(start_offset / (in.units + p.joining), p.heads - 1);       // below it, unless the lengths have changed
-  in.of->h = start_h;
-  in.of->kv = start_h / p.tiles;
   in.tile = start_offset - start_h * (in.units + p.joining);
+  *in.of = Sequence{start_b, start_h, start_h / p.tiles, start_slot, start_tokens};
+  __syncwarp();
   settle(in);                          // a run that begins with a joining step leaves it to the owner of the sequence's last unit
   Cursor at = in;
   at.of = &sequences[1][warp];
   *at.of = *in.of;
+  __syncwarp();
   if (threadIdx.x == 0) {
     // A run that begins inside a sequence, the first one to: the parts are the last of the run before (its first, if that begins
     // with the sequence, or with the joining step before it), and the first of every run from this one to the owner of the sequence's last unit.
