@@ -325,3 +325,18 @@ def test_refusals_without_a_gpu():
                         (dict(x=264), 3), (dict(x_stride=60), 3), (dict(codes=260), 3), (dict(slots=1), 1), (dict(slots=-1), 1),
                         (dict(slots=1, wr=256, wrs=256), 1), (dict(slots=1, wr=256, wrs=256, dense=1, n=130), 2), (dict(entries=-1), 1)):
         assert lib.tw_matvec(ctypes.byref(_lib.MatvecArgs(**(ok | bad))), None) == status, bad
+
+
+@gpu
+@pytest.mark.parametrize('r,n,k', [(1, 2, 5024), (3, 1, 5024), (2, 3, 544), (1, 2, 576), (2, 5, 608), (9, 4, 4640), (1, 7, 672), (8, 129, 1184)])
+def test_scales_that_end_with_their_last_row(r, n, k):
+    """K with a remainder: the words that a quad of K128 blocks copies lie within the scales, which NaN bytes follow here."""
+    from thunderworld_b200 import ops
+    codes, scales = weights(n, k, n + k)
+    held = torch.full((n * k // 16 + 64,), 0x7f, device='cuda', dtype=torch.uint8)
+    held[:n * k // 16] = scales.view(torch.uint8).flatten()
+    behind = held[:n * k // 16].view(torch.float8_e4m3fn).view(n, k // 16)
+    x, factor = rows_of(r, k, r), torch.tensor(3e-4, device='cuda')
+    y = ops.fp4_matvec(x, codes, behind, factor)
+    check(y, x, decoded(codes, scales), factor)
+    assert torch.equal(y, ops.fp4_matvec(x, codes, scales, factor))

@@ -181,6 +181,8 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_kernel(const __grid_constan
   const bool fifth = scale_pitch % 8 && lane < 16;
   // lanes whose 32 k of the last block lie behind K repeat the block's first 32 (x is zero there)
   const int last_block = p.kb - 1 - kb0, tail = last_block < nkb && (kb0 + last_block) * 128 + t * 32 >= p.k ? t * 16 : 0;
+  // quads before this block have all their words within their rows: four blocks, and where there is a fifth word, another that it lies in
+  const int whole = last_block - (scale_pitch % 8 ? 4 : 3);
   const uint8_t *c0, *c8, *s0, *s32;               // where the round's next quad begins for this lane
   auto aligned = [](const uint8_t* at) { return reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(at) & ~(uintptr_t)7); };
   auto point = [&]() {
@@ -194,7 +196,7 @@ __global__ void __launch_bounds__(THREADS, 2) matvec_kernel(const __grid_constan
     const int n = width(in);
     const uint32_t offset = slot * QUAD;
     if (n > 0 && (!BANK || in.at < in.w0)) {
-      if (n == 4 && in.at + 3 < last_block) {                        // the usual quad
+      if (n == 4 && in.at < whole) {                                 // the usual quad
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           copy16(code_to + offset + j * 1024, c0 + j * 64);
