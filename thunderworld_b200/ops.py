@@ -10,6 +10,7 @@ Host-side mirror of the reference's packers and launch wrappers:
 torch is used for device memory and streams only.
 """
 import ctypes
+import threading
 from contextlib import nullcontext
 from dataclasses import dataclass
 from functools import lru_cache
@@ -57,8 +58,10 @@ def _device(device):
 # Scratch per stream: calls on one stream run one after the other. A call that is being captured gets scratch of its own graph's, so
 # that two graphs captured on one stream may be replayed side by side; only the newest capture's is held here, older ones live as
 # long as their graph's pool. 'zeroed' is 8 bytes that kernels leave zeroed (the graph zeroes its own on every replay), 'paged'
-# needs no initialisation and grows as wanted.
+# needs no initialisation and grows as wanted. A call of two launches has its plan in the scratch between them, so threads take turns
+# from the lookup to the last launch (`_launching`; ctypes lets other threads run meanwhile).
 _stream_scratch = {}
+_launching, _making = threading.Lock(), threading.Lock()
 
 
 def _scratch(device, stream, kind='zeroed', nbytes=8):
@@ -66,8 +69,11 @@ def _scratch(device, stream, kind='zeroed', nbytes=8):
     key = (device, stream, kind, capture != 0)
     held = _stream_scratch.get(key)
     if held is None or held[0] != capture or held[1].numel() < nbytes:
-        make = torch.zeros if kind == 'zeroed' else torch.empty
-        held = _stream_scratch[key] = (capture, make(nbytes, device=device, dtype=torch.uint8))
+        with _making:                                             # two threads that both find none share one
+            held = _stream_scratch.get(key)
+            if held is None or held[0] != capture or held[1].numel() < nbytes:
+                make = torch.zeros if kind == 'zeroed' else torch.empty
+                held = _stream_scratch[key] = (capture, make(nbytes, device=device, dtype=torch.uint8))
     return held[1]
 
 
@@ -307,10 +313,13 @@ def _cache_status(device):
     """Address of the device word that the paged operators report in (device_status reads it; it lives as long as the process)."""
     word = _status_words.get(device)
     if word is None:
-        word = _workspace(device, 256, 'c').data_ptr()
-        if not torch.cuda.is_current_stream_capturing():
-            torch.cuda.current_stream(device).synchronize()       # zeroed before another stream's call may write it
-        _status_words[device] = word
+        with _making:
+            word = _status_words.get(device)
+            if word is None:
+                word = _workspace(device, 256, 'c').data_ptr()
+                if not torch.cuda.is_current_stream_capturing():
+                    torch.cuda.current_stream(device).synchronize()       # zeroed before another stream's call may write it
+                _status_words[device] = word
     return word
 
 
@@ -417,7 +426,7 @@ def paged_attention(q, k_pages, v_pages, table, lengths, *, slots=None, scale=No
         raise ValueError('out must not share memory with q')
     lse = q.new_empty((batch, hq), dtype=torch.float32) if return_lse else None
     lib = _lib.load()
-    with _device(dev):
+    with _device(dev), _launching:
         stream = _stream(dev)
         scratch = _scratch(dev, stream, 'paged', _scratch_bytes('tw_paged_attention_workspace', batch, hq, hk, dim, width * page))
         args = _lib.PagedAttentionArgs(
@@ -493,7 +502,7 @@ def cache_append_(k, v, k_pages, v_pages, table, lengths, refs, *, slots=None, c
         if (at < k_end and k_at < end) or (at < v_end and v_at < end):
             raise ValueError('k and v must not lie in the pages')
     call = _lib.AppendArgs(new_k, new_v, _ptr(slots), _ptr(cu), _ptr(k_scale), _ptr(v_scale), ks[0], ks[1], vs[0], vs[1], batch, rows)
-    with _device(dev):
+    with _device(dev), _launching:
         stream = _stream(dev)
         scratch = _scratch(dev, stream, 'paged', _scratch_bytes('tw_cache_append_workspace', batch, rows))
         _lib.check(_lib.load().tw_cache_append(ctypes.byref(args), ctypes.byref(call), scratch.data_ptr(), stream))
@@ -511,7 +520,7 @@ def cache_fork_(k_pages, v_pages, table, lengths, refs, parents, children):
         raise ValueError('one child per parent is required')
     if not count:
         return
-    with _device(dev):
+    with _device(dev), _launching:
         stream = _stream(dev)
         scratch = _scratch(dev, stream, 'paged', _scratch_bytes('tw_cache_fork_workspace', count))
         _lib.check(_lib.load().tw_cache_fork(ctypes.byref(args), parents.data_ptr(), children.data_ptr(), count, scratch.data_ptr(), stream))
@@ -532,7 +541,7 @@ def cache_compact_(k_pages, v_pages, table, lengths, refs):
     and refs, and returns live as an int32 scalar tensor."""
     args, dev, *_ = _cache(k_pages, v_pages, table, lengths, refs)
     live = torch.empty((), device=dev, dtype=torch.int32)
-    with _device(dev):
+    with _device(dev), _launching:
         stream = _stream(dev)
         scratch = _scratch(dev, stream, 'paged', _scratch_bytes('tw_cache_compact_workspace', refs.numel()))
         _lib.check(_lib.load().tw_cache_compact(ctypes.byref(args), live.data_ptr(), scratch.data_ptr(), stream))
