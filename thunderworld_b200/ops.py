@@ -316,8 +316,10 @@ def _cache_status(device):
         with _making:
             word = _status_words.get(device)
             if word is None:
-                word = _workspace(device, 256, 'c').data_ptr()
-                if not torch.cuda.is_current_stream_capturing():
+                with _device(device):
+                    if torch.cuda.is_current_stream_capturing():          # the word would be the graph's, and zero at every replay
+                        raise RuntimeError('the first call of a paged operator on a device cannot be captured: make a PagedCache or call one before')
+                    word = _workspace(device, 256, 'c').data_ptr()
                     torch.cuda.current_stream(device).synchronize()       # zeroed before another stream's call may write it
                 _status_words[device] = word
     return word
@@ -396,7 +398,7 @@ def paged_attention(q, k_pages, v_pages, table, lengths, *, slots=None, scale=No
     128; table int32 [sequences, pages per sequence], lengths int32 [sequences], slots int32 [batch], all read on the device:
     no host synchronisation. scale defaults to dim ** -0.5. Returns bf16 [batch, heads, dim], with return_lse also the float32
     natural log of each softmax's sum (-inf and zeros for an empty sequence). Sums are 32 bits wide. Slots, lengths and table entries
-    that lead outside are left out and reported by device_status()."""
+    that lead outside are left out and reported by device_status(). Can be captured, except for a device's first paged call."""
     pages, hk, page, dim, fp8, ks, vs = _check_pages(k_pages, v_pages)
     dev = k_pages.device
     if q.ndim != 3 or q.dtype is not torch.bfloat16 or q.device != dev or q.shape[2] != dim or q.stride(2) != 1:
