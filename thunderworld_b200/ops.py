@@ -594,10 +594,11 @@ def _check_bf16(*tensors):
 
 
 def _stats(device, want):
-    """(stats[2] float32, scratch) or (None, None). The scratch word pair is zeroed once per device."""
+    """(stats[2] float32, scratch) or (None, None). The scratch is the stream's, or the capture's: a maximum and a ticket that calls
+    on two streams must not share."""
     if not want:
         return None, None
-    return torch.empty(2, device=device, dtype=torch.float32), _workspace(device, 8, 'pointwise')
+    return torch.empty(2, device=device, dtype=torch.float32), _scratch(device, _stream(device))
 
 
 def activate_with_factor(a, b=None, *, mode=None, want_factor=True, return_stats=False):
