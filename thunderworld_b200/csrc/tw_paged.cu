@@ -13,7 +13,10 @@
 // by the values on the tensor cores (m16n8k16, 32-bit sums); warps meet only at the end of a sequence. With bf16 pages a
 // probability is two bf16 values (8 + 8 bits), so that rounding it adds nothing to the result's own rounding (an infinite value
 // then gives NaN, since the second may be zero or negative); with E4M3 pages both
-// products are in f16, which holds E4M3 exactly, and q is scaled by a power of two per head to the range of f16.
+// products are in f16, which holds E4M3 exactly, and q is scaled by a power of two per head to the range of f16. There a probability is
+// one f16 value, 2^15 times itself: rounded by 2^-12 of itself, a sixteenth of the result's own rounding (a second value would double the
+// products of values), and of what lies 2^-29 and more below the warp's running maximum by 2^-40 of that; without the factor everything
+// 2^-25 below was lost, where a key with all the weight and a value of zero leaves the result to such tokens.
 // Tokens behind a sequence's end, and those of a table entry outside the pool (reported in the status word), are masked
 // and read as zeros, whatever lies there.
 //
@@ -105,8 +108,16 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// What probabilities and their sums are multiplied by, as a power of two; the sums of parts carry it to the end, where it cancels.
+__host__ __device__ constexpr int p_shift(bool fp8) { return fp8 ? 15 : 0; }
 // Weight of a part whose maximum is m among parts whose largest is top; nothing is left of a part without tokens.
 __device__ __forceinline__ float weight_of(float m, float top) { return m == -INFINITY ? 0.f : exp2_fast(m - top); }
+
+// Natural log of a softmax's sum, from the maximum and the sum in base 2.
+template <bool FP8>
+__device__ __forceinline__ float lse_of(float top, float sum) {
+  return sum == 0.f ? -INFINITY : (top + log2f(sum * (1.f / (1 << p_shift(FP8))))) * 0.693147180559945f;
+}
 
 // Place of 16-byte chunk c of row r in a tile of rows of CHUNKS chunks: what eight lanes read at once lies in different banks.
 template <int CHUNKS> __device__ __forceinline__ int swizzled(int c, int r) { return CHUNKS == 4 ? c ^ (r >> 1 & 3) : c ^ (r & 7); }
@@ -440,7 +451,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, WIDE)) paged_attention
             for (int n = 0; n < D / 8; ++n) { o[n][2 * h] *= a; o[n][2 * h + 1] *= a; }
           }
         }
-        const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+        const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0] - p_shift(FP8), m[1] == -INFINITY ? 0.f : m[1] - p_shift(FP8)};
 #pragma unroll
         for (int u = 0; u < SUBS; ++u) {
           uint32_t hi[4] = {}, lo[4] = {};                // probabilities as an A fragment: rows g, g + 8; tokens 2 t, 2 t + 8
@@ -535,7 +546,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, WIDE)) paged_attention
             if (whole) {
               const long long head = (long long)at.of->b * p.hk * p.group + kv * p.group + row0 + r;
               p.out[head * D + d] = __float2bfloat16_rn(ml.y == 0.f ? 0.f : y * v_scale / ml.y);
-              if (p.lse && d == 0) p.lse[head] = ml.y == 0.f ? -INFINITY : (ml.x + log2f(ml.y)) * 0.693147180559945f;
+              if (p.lse && d == 0) p.lse[head] = lse_of<FP8>(ml.x, ml.y);
             } else {
               const long long slot = ((long long)blockIdx.x * 2 + (first_segment ? 0 : 1)) * p.rows + r;
               p.part_o[slot * D + d] = y;
@@ -554,7 +565,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, WIDE)) paged_attention
 // Joins what several CTAs have of one (sequence, head tile): a block per border between two runs and query row, whose warps take the
 // parts in turn. (One row and eight warps a block: 1 x 3840 tokens 14.7 us in all; four rows and four warps each 15.6, sixteen warps 14.8.)
 constexpr int JOIN_WARPS = 8;
-template <int D>
+template <int D, bool FP8>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const __grid_constant__ Params p) {
   constexpr int VEC = D / 32;                              // channels of a lane
   struct __align__(VEC * 4) Channels { float v[VEC]; };
@@ -596,11 +607,11 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) paged_join_kernel(const __gri
     for (int j = 0; j < VEC; ++j) y.v[j] += sums[q][lane].v[j];
   const long long head = border.z + r;
   const int kv = (border.z / p.group) % p.hk;
-  const float scale = sum == 0.f ? 0.f : (p.v_scale ? __ldg(p.v_scale + kv) : 1.f) / sum;
+  const float scale = p.v_scale ? __ldg(p.v_scale + kv) : 1.f;
 #pragma unroll
   for (int j = 0; j < VEC; j += 2)
-    *reinterpret_cast<uint32_t*>(p.out + head * D + lane * VEC + j) = sum == 0.f ? 0u : pack_bf16(y.v[j] * scale, y.v[j + 1] * scale);
-  if (p.lse && lane == 0) p.lse[head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.693147180559945f;
+    *reinterpret_cast<uint32_t*>(p.out + head * D + lane * VEC + j) = sum == 0.f ? 0u : pack_bf16(y.v[j] * scale / sum, y.v[j + 1] * scale / sum);
+  if (p.lse && lane == 0) p.lse[head] = lse_of<FP8>(top, sum);
 }
 
 int part_rows(int hq, int hk) { return hq / hk < 16 ? hq / hk : 16; }
@@ -637,7 +648,7 @@ int launch(const Params& p, cudaStream_t stream) {
   early.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &early;
   config.numAttrs = 1;
-  if (cudaLaunchKernelEx(&config, paged_join_kernel<D>, p) != cudaSuccess) { (void)cudaGetLastError(); return TW_ERR_LAUNCH; }
+  if (cudaLaunchKernelEx(&config, paged_join_kernel<D, FP8>, p) != cudaSuccess) { (void)cudaGetLastError(); return TW_ERR_LAUNCH; }
   return TW_OK;
 }
 
