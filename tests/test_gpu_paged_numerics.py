@@ -1,4 +1,4 @@
-"""Attention over a paged cache where probabilities are far apart, against the formula in 64 bits.
+"""Attention over a paged cache where probabilities are far apart and where values are infinite, against the formula in 64 bits.
 
 Tolerances, as for the other tests of this operator: scores off by A (their 32-bit sums), a probability by a relative 2 A + 2^-20 more
 for the exponential and its argument, and by its rounding: 2^-16 with bf16 pages (two bf16 values, the first truncated), with E4M3
@@ -94,3 +94,25 @@ def test_many_tokens_far_below_one(fp8):
     kp, vp, table, lengths = cache_of(k, v, 64, 2)
     out, lse = ops.paged_attention(q, kp, vp, table, lengths, scale=1., return_lse=True)
     check(out, lse, q, k, v, 1., fp8)
+
+
+@gpu
+@pytest.mark.parametrize('hq,hk,dim', [(4, 2, 128), (16, 1, 128), (8, 1, 64), (24, 1, 64)])
+@pytest.mark.parametrize('tokens', [1, 16, 50, 2000])
+def test_infinite_values(hq, hk, dim, tokens):
+    """bf16 values of +inf, -inf and both in one channel: the formula's infinity or NaN, and every other channel as without them."""
+    from thunderworld_b200 import ops
+    g = torch.Generator().manual_seed(tokens)
+    q = torch.randn(3, hq, dim, generator=g).bfloat16().cuda()
+    k, v = torch.randn(2, 3, hk, tokens, dim, generator=g).bfloat16().cuda()
+    at = [int(i) for i in torch.randint(0, tokens, (4,), generator=g)]
+    clean = ops.paged_attention(q, *cache_of(k, v, 16, 3))
+    v[0, 0, at[0], 5] = math.inf
+    v[1, 0, at[1], 40] = -math.inf
+    v[2, hk - 1, at[2], 9], v[2, hk - 1, (at[2] + 1) % tokens, 9] = math.inf, -math.inf
+    out = ops.paged_attention(q, *cache_of(k, v, 16, 3))
+    p, *_ = formula(q, k, v, dim ** -.5)
+    want = (p[..., None] * v.double()[:, :, None]).sum(-2).view(3, hq, dim)
+    odd = ~want.isfinite()
+    assert odd.sum() == 3 * hq // hk and torch.equal(out[odd].double().nan_to_num(7., 8., 9.), want[odd].nan_to_num(7., 8., 9.))
+    assert torch.equal(out[~odd], clean[~odd])

@@ -11,8 +11,9 @@
 // A warp takes 16 (32) of a unit's tokens: it copies their rows (two units ahead) to a ring of its own, multiplies q (the group's heads,
 // padded to 16 rows) by the keys, keeps its own running maximum and sum in 32 bits, base 2, and multiplies the probabilities
 // by the values on the tensor cores (m16n8k16, 32-bit sums); warps meet only at the end of a sequence. With bf16 pages a
-// probability is two bf16 values (8 + 8 bits), so that rounding it adds nothing to the result's own rounding (an infinite value
-// then gives NaN, since the second may be zero or negative); with E4M3 pages both
+// probability is two bf16 values (8 bits each, off by at most 2^-16 of it), so that rounding it adds nothing to the result's own rounding.
+// Both are positive (the first is truncated, the second has 2^-24 of the first added), so that an infinite value gives that infinity, as its
+// product with the probability does (NaN where that is below 2^-109 of the warp's running maximum). With E4M3 pages both
 // products are in f16, which holds E4M3 exactly, and q is scaled by a power of two per head to the range of f16. There a probability is
 // one f16 value, 2^15 times itself: rounded by 2^-12 of itself, a sixteenth of the result's own rounding (a second value would double the
 // products of values), and of what lies 2^-29 and more below the warp's running maximum by 2^-40 of that; without the factor everything
@@ -149,6 +150,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, WIDE)) paged_attention
   constexpr int SUB = 16 * ROW, TILE = SUBS * SUB;         // bytes of 16 tokens' rows, of a tile's
   constexpr uint32_t ALL = TOK == 32 ? 0xffffffffu : 0xffffu;
   constexpr int STAGES = 2, HALVES = WIDE ? 2 : 1;
+  constexpr float LESS = -1.f + 1.f / (1 << 24);           // x + LESS hi: what is left of x, and 2^-24 hi
   extern __shared__ __align__(128) uint8_t dynamic[];                             // [WARPS][STAGES][K, V][TOK rows], from a multiple of 256
   __shared__ float gather[WARPS * JOIN_ROWS * D];
   __shared__ float part_m[WARPS][16], part_l[WARPS][16];
@@ -464,8 +466,9 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, WIDE)) paged_attention
               if (FP8) {
                 hi[i] = pack_f16(x, y);
               } else {
-                hi[i] = pack_bf16(x, y);
-                lo[i] = pack_bf16(x - tw::bf16_bits_to_float(hi[i] & 0xffffu), y - tw::bf16_bits_to_float(hi[i] >> 16));
+                const uint32_t xb = __float_as_uint(x), yb = __float_as_uint(y);
+                hi[i] = __byte_perm(xb, yb, 0x7632);
+                lo[i] = pack_bf16(__fmaf_rn(__uint_as_float(xb & 0xffff0000u), LESS, x), __fmaf_rn(__uint_as_float(yb & 0xffff0000u), LESS, y));
               }
             }
           }
