@@ -223,9 +223,10 @@ int tw_paged_attention(const TwPagedAttentionArgs* args, void* stream);
 
 /* ---- pages of a key-value cache ------------------------------------------------------------------
  * State on the device: table [sequences, max_pages] (page numbers, -1 behind a sequence's pages), lengths [sequences] (tokens), refs
- * [pages] (sequences that hold a page, 0: free). All calls are asynchronous and can be captured. append, fork and compact change
+ * [pages] (sequences that hold a page, 0: free). All calls are asynchronous and can be captured. append and fork change
  * nothing when they cannot be done, and raise *status to "a page table entry, slot or length leads outside the cache" or "the
- * page pool or a sequence's table is full"; free leaves out what leads outside, and reports it. sequences <= 65536. The two pools
+ * page pool or a sequence's table is full"; free and compact leave out what leads outside, and report it. The entries that an append
+ * relies on are those of partly filled last pages, a fork relies on all of its parents'. sequences <= 65536. The two pools
  * share no memory, and the rows that append reads lie outside them. */
 typedef struct TwCache {
   void *k_pages, *v_pages;       /* [pages, hk, page, dim], rows contiguous, bf16 or (fp8) E4M3, 16-byte aligned heads */

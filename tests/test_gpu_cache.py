@@ -377,3 +377,90 @@ def test_refusals_without_a_gpu():
     assert lib.tw_cache_fork(ref(c), None, 256, 1, 256, None) == 1 and lib.tw_cache_fork(ref(c), 256, 256, 0, 256, None) == 1
     assert lib.tw_cache_free(ref(c), 256, 0, None) == 1 and lib.tw_cache_compact(ref(c), None, None, None) == 1
     assert lib.tw_cache_append_workspace(0, 1) == 0 and lib.tw_cache_fork_workspace(0) == 0 and lib.tw_cache_compact_workspace(0) == 0
+
+
+@gpu
+@pytest.mark.parametrize('entry', [-1, -2 ** 31, 9, 2 ** 31 - 1])
+def test_a_bad_entry_of_the_last_page_leaves_an_append_undone(entry):
+    """The page that the next row belongs to is not in the pool: no length, page or row changes, for the sequences beside it neither."""
+    from thunderworld_b200 import ops
+    cache = make(9, 4, 1, 64, False, sequences=4, tokens=32)
+    x = torch.randn(20, 1, 64, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    cache.append(x, x, i32([0, 1]), i32([0, 6, 14]))       # 2 pages, the second torn; 2 full pages
+    cache.table[0, 1] = entry
+    model = Model(cache)
+    cache.append(x, x, i32([0, 2]), i32([0, 1, 8]))
+    assert ops.device_status() == 11
+    model.same(cache)
+    ops.reset_device_status()
+    cache.append(x, x, i32([0, 1, 2]), i32([0, 0, 3, 8]))  # no row for that sequence, which is then not looked at
+    model.append(x, x, [1, 2], [0, 3, 8])
+    model.same(cache)
+    cache.check()
+    cache.table[1, 1] = entry                              # a full page that no new row lies in
+    model.table[1][1] = entry
+    cache.append(x, x, i32([1]), i32([0, 1]))
+    model.append(x, x, [1], [0, 1])
+    model.same(cache)
+    cache.check()
+
+
+@gpu
+@pytest.mark.parametrize('entry', [-1, -2 ** 31, 40, 2 ** 31 - 1])
+@pytest.mark.parametrize('at', [0, 3, 6])
+@pytest.mark.parametrize('count', [1, 2, 5])
+def test_a_bad_entry_of_a_parent_leaves_a_fork_undone(entry, at, count):
+    """A full page (0, 3) or the torn last one (6) of one of the parents is not in the pool: no child is made, no count raised."""
+    from thunderworld_b200 import ops
+    cache = make(40, 4, 2, 64, False, sequences=12, tokens=64)
+    x = torch.randn(40, 2, 64, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    cache.append(x, x, i32([0, 1]), i32([0, 27, 36]))      # 7 and 3 pages, both with a torn one
+    good = int(cache.table[0, at])
+    cache.table[0, at] = entry
+    model = Model(cache)
+    cache.fork(i32(([1] * (count - 1) + [0])), i32(range(2, 2 + count)))
+    assert ops.device_status() == 11
+    model.same(cache)
+    ops.reset_device_status()
+    cache.table[0, at] = model.table[0][at] = good
+    cache.table[0, 7] = entry                              # behind the sequence's pages: nobody's
+    model.table[0][7] = entry
+    cache.fork(i32([1, 0]), i32([3, 2]))
+    model.fork([1, 0], [3, 2])
+    model.same(cache)
+    cache.check()
+
+
+@gpu
+def test_forks_of_more_sequences_than_threads():
+    from thunderworld_b200 import ops
+    cache = make(3000, 2, 1, 64, False, sequences=2700, tokens=20)
+    x = torch.randn(1300 * 3, 1, 64, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    cache.append(x[:3900], x[:3900], i32(range(1300)), i32(range(0, 3901, 3)))
+    good, before = int(cache.table[1290, 0]), [t.clone() for t in (cache.table, cache.lengths, cache.refs)]
+    cache.table[1290, 0] = 3000
+    cache.fork(i32(range(100, 1300)), i32(range(1300, 2500)))
+    assert ops.device_status() == 11
+    ops.reset_device_status()
+    cache.table[1290, 0] = good
+    assert all(torch.equal(a, b) for a, b in zip(before, (cache.table, cache.lengths, cache.refs)))
+    cache.fork(i32(range(100, 500)), i32(range(1300, 1700)))
+    assert ops.device_status() == 0 and torch.equal(cache.table[1300:1700, 0], cache.table[100:500, 0])
+    assert cache.table[1300:1700, 1].tolist() == list(range(2600, 3000)) and (cache.lengths[1300:1700] == 3).all()
+
+
+@gpu
+@pytest.mark.parametrize('entry', [-1, 40, 2 ** 31 - 1])
+def test_compact_leaves_a_bad_entry_as_it_is(entry):
+    """And reports it; the good ones' pages move, and are found, all the same."""
+    from thunderworld_b200 import ops
+    cache = make(40, 4, 2, 64, False, sequences=6, tokens=64)
+    x = torch.randn(60, 2, 64, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    cache.append(x, x, i32([0, 1, 2]), i32([0, 20, 39, 60]))
+    cache.free(i32([0]))
+    cache.table[1, 2] = entry
+    model = Model(cache)
+    assert int(cache.compact()) == model.compact()
+    assert ops.device_status() == 11
+    ops.reset_device_status()
+    model.same(cache)

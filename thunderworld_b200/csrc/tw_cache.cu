@@ -7,7 +7,8 @@
 // append, fork and compact are two launches: a plan by one CTA (a few kilobytes of counts and, only where a page is needed,
 // one pass over refs: block-wide prefix sums give every request its page, so the result does not depend on any order of execution),
 // then the copies by the whole device, which is what takes the time where there is much to copy (HBM-bound, 16 bytes a lane). A call whose
-// plan does not work out (an entry outside, a slot twice, a full pool) changes nothing and reports it in the status word.
+// append or fork does not work out (a slot, length or page outside, a slot twice, a full pool) changes nothing and reports it in the status
+// word; compact leaves table entries outside the pool as they are and reports them.
 // Measured (B200): compact's copies of 91 MB of pages (64 tokens, 8 heads of 128, bf16) 27.1 us, 6.6 TB/s read and written; append and fork
 // of tens of sequences copy a microsecond or two: they are held by their two launches.
 #include "tw_common.cuh"
@@ -28,6 +29,7 @@ struct Plan { int ok, count, live, unused; };                         // head of
 
 __device__ __forceinline__ int pages_of(const Cache& c, int tokens) { return (tokens + (1 << c.page_shift) - 1) >> c.page_shift; }
 __device__ __forceinline__ void report(const Cache& c, int code) { if (c.status) atomicMax(c.status, code); }
+__device__ __forceinline__ bool outside(const Cache& c, int page) { return page < 0 || page >= c.pages; }
 __device__ __forceinline__ long long capacity(const Cache& c) { return (long long)c.max_pages << c.page_shift; }
 
 // Exclusive prefix sum of one value per thread of the planning CTA; returns the sum of all in `total`.
@@ -100,6 +102,7 @@ __global__ void __launch_bounds__(PLAN) append_plan_kernel(const __grid_constant
         const int before = c.lengths[s];
         if (before < 0 || before > capacity(c)) wrong = TW_ERR_PAGE;
         else if (before + (long long)(to - from) > capacity(c)) wrong = TW_ERR_CACHE_FULL;
+        else if (to > from && before & ((1 << c.page_shift) - 1) && outside(c, c.table[s * c.table_stride + (before >> c.page_shift)])) wrong = TW_ERR_PAGE;
         else { need = pages_of(c, before + to - from) - pages_of(c, before); a.base[i] = before; }
       }
       if (wrong) { atomicMax(&error, wrong); need = 0; }
@@ -160,7 +163,7 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const __grid_constant_
       if (r < a.cu[i] || r >= a.cu[i + 1]) continue;                   // rows of no entry
     }
     const int pos = a.base[i] + (a.cu ? r - a.cu[i] : 0), page = c.table[slot_of(a, i) * c.table_stride + (pos >> c.page_shift)];
-    if (page < 0 || page >= c.pages) { report(c, TW_ERR_PAGE); continue; }
+    if (outside(c, page)) { report(c, TW_ERR_PAGE); continue; }        // not after the plan, unless somebody changes the table meanwhile
     const uint4 k = *reinterpret_cast<const uint4*>(a.k + r * a.k_row + head * a.k_head + at), v = *reinterpret_cast<const uint4*>(a.v + r * a.v_row + head * a.v_head + at);
     const long long row = (long long)(pos & ((1 << c.page_shift) - 1)) * c.row + at * (FP8 ? 1 : 2);
     uint8_t *ko = c.k + page * c.k_page + head * c.k_head + row, *vo = c.v + page * c.v_page + head * c.v_head + row;
@@ -204,6 +207,20 @@ __global__ void __launch_bounds__(PLAN) fork_plan_kernel(const __grid_constant__
     const int rank = block_scan(need, total);
     if (i < f.count) f.fresh[i] = need ? -2 - (needed + rank) : -1;      // the request, until its page is known
     needed += total;
+  }
+  __syncthreads();
+  if (!error) {
+    // the parents' pages have to be pages: as many threads look through one's as there are for each
+    int each = PLAN;
+    while (each > 1 && each * f.count > PLAN) each >>= 1;
+    bool wrong = false;
+    for (int i = threadIdx.x / each; i < f.count; i += PLAN / each) {
+      const int* row = c.table + f.parents[i] * c.table_stride;
+      const int pages = pages_of(c, f.tokens[i]);
+#pragma unroll 4
+      for (int j = threadIdx.x % each; j < pages; j += each) wrong = wrong | outside(c, row[j]);
+    }
+    if (wrong) atomicMax(&error, (int)TW_ERR_PAGE);
   }
   __syncthreads();
   int* free_pages = f.fresh + f.count;
@@ -250,13 +267,13 @@ __global__ void __launch_bounds__(128) fork_copy_kernel(const __grid_constant__ 
     for (int j = threadIdx.x; j < full; j += 128) {
       const int page = from[j];
       to[j] = page;
-      if (page >= 0 && page < c.pages) atomicAdd(c.refs + page, 1); else report(c, TW_ERR_PAGE);
+      if (outside(c, page)) report(c, TW_ERR_PAGE); else atomicAdd(c.refs + page, 1);       // as above
     }
     if (threadIdx.x == 0 && part) to[full] = fresh;
   }
   if (!part) return;
   const int old = from[full];
-  if (old < 0 || old >= c.pages) { if (threadIdx.x == 0) report(c, TW_ERR_PAGE); return; }
+  if (outside(c, old)) { if (threadIdx.x == 0) report(c, TW_ERR_PAGE); return; }
   for (int p = blockIdx.y; p < 2 * c.hk; p += gridDim.y) {
     const int head = p >> 1;
     const long long page = p & 1 ? c.v_page : c.k_page, at = head * (p & 1 ? c.v_head : c.k_head);
@@ -278,7 +295,7 @@ __global__ void __launch_bounds__(128) free_kernel(const __grid_constant__ Cache
   for (int j = threadIdx.x; j < pages; j += 128) {
     const int page = row[j];
     row[j] = -1;
-    if (page < 0 || page >= c.pages) report(c, TW_ERR_PAGE);
+    if (outside(c, page)) report(c, TW_ERR_PAGE);
     else if (atomicSub(c.refs + page, 1) <= 0) { atomicAdd(c.refs + page, 1); report(c, TW_ERR_PAGE); }     // nobody held it
   }
 }
@@ -318,7 +335,7 @@ __global__ void __launch_bounds__(256) compact_move_kernel(const __grid_constant
     if (tokens <= 0 || (long long)j << c.page_shift >= tokens) continue;
     int* at = c.table + s * c.table_stride + j;
     const int page = *at;
-    if (page < 0 || page >= c.pages) report(c, TW_ERR_PAGE);
+    if (outside(c, page)) report(c, TW_ERR_PAGE);
     else if (page >= live) {
       const int to = m.number[page];
       if (to >= 0 && to < live) *at = to; else report(c, TW_ERR_PAGE);

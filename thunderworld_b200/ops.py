@@ -468,7 +468,8 @@ def cache_append_(k, v, k_pages, v_pages, table, lengths, refs, *, slots=None, c
     """New tokens behind their sequences: rows k, v bf16 [rows, kv_heads, dim] go to the cache, row i behind the tokens of slot
     slots[i] (i by default), or with cu int32 [batch + 1] rows cu[i] ... cu[i + 1] - 1. New pages are the lowest free numbers, in the
     order of i; table, lengths and refs are updated. A slot may be named once. E4M3 pages hold k / k_scale[head] rounded, saturating.
-    All on the device: a call that cannot be done (a full pool or table, an index outside) changes nothing and shows in device_status()."""
+    All on the device: a call that cannot be done (a full pool or table; a slot, length or partly filled last page outside) changes
+    nothing and shows in device_status()."""
     args, dev, hk, dim, fp8, sequences = _cache(k_pages, v_pages, table, lengths, refs)
     shape = k.shape
     if len(shape) != 3 or shape != v.shape or shape[1] != hk or shape[2] != dim or k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 \
@@ -513,7 +514,8 @@ def cache_append_(k, v, k_pages, v_pages, table, lengths, refs, *, slots=None, c
 def cache_fork_(k_pages, v_pages, table, lengths, refs, parents, children):
     """Slot children[i], which must be empty and may be named once, becomes a copy of slot parents[i] as it was before the call: full
     pages are shared (refs counts their holders), the rows of a partly filled last page are copied to the lowest free page. int32 [n]
-    each. A call that cannot be done changes nothing and shows in device_status()."""
+    each. A call that cannot be done (a full pool; a slot, length or page of a parent outside) changes nothing and shows in
+    device_status()."""
     args, dev, *_ = _cache(k_pages, v_pages, table, lengths, refs)
     _check_int32(dev, 'parents', parents)
     _check_int32(dev, 'children', children)
@@ -540,7 +542,7 @@ def cache_free_(table, lengths, refs, slots, page_size):
 
 def cache_compact_(k_pages, v_pages, table, lengths, refs):
     """Moves the live pages to the numbers 0 ... live - 1 (the r-th live page at or above live to the r-th free one below), updates table
-    and refs, and returns live as an int32 scalar tensor."""
+    and refs, and returns live as an int32 scalar tensor. A table entry outside the pool stays as it is and shows in device_status()."""
     args, dev, *_ = _cache(k_pages, v_pages, table, lengths, refs)
     live = torch.empty((), device=dev, dtype=torch.int32)
     with _device(dev), _launching:
