@@ -150,6 +150,9 @@ typedef struct TwMatvecArgs {
   int32_t out_f32;          /* 0: bf16, else float32 */
 } TwMatvecArgs;
 int tw_matvec(const TwMatvecArgs* args, void* stream);
+/* Launches of such a call, an even share of the rows each: more than one where the rows' part of K does not fit an SM's shared memory. 0:
+ * sizes that are refused. Pure host function. */
+int tw_matvec_launches(int rows, int k, int bank);
 
 /* ---- streaming FP4 attention -----------------------------------------------------------------
  * Three calls replace the reference's attention launch chain (thunderworld_fp4/runtime.py:32-108):

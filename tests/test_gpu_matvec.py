@@ -340,3 +340,35 @@ def test_scales_that_end_with_their_last_row(r, n, k):
     y = ops.fp4_matvec(x, codes, behind, factor)
     check(y, x, decoded(codes, scales), factor)
     assert torch.equal(y, ops.fp4_matvec(x, codes, scales, factor))
+
+
+@gpu
+@pytest.mark.parametrize('r,n,k', [(29, 130, 16384), (30, 130, 16384), (21, 256, 24576), (22, 256, 24576), (16, 70, 32768), (17, 70, 32768), (31, 33, 14368), (32, 33, 14368),
+                                   (20, 300, 15392)])
+def test_rows_on_both_sides_of_what_fits_at_once(r, n, k):
+    """Sizes at which the rows go from one launch to two."""
+    from thunderworld_b200 import ops
+    codes, scales = weights(n, k, n + k)
+    x, factor = rows_of(r, k, r), torch.tensor(3e-4, device='cuda')
+    check(ops.fp4_matvec(x, codes, scales, factor), x, decoded(codes, scales), factor)
+
+
+@gpu
+@pytest.mark.parametrize('r,n,k', [(28, 128, 16384), (29, 128, 16384), (20, 256, 24576), (21, 256, 24576), (15, 128, 32768), (16, 128, 32768), (32, 256, 32768)])
+def test_rows_on_both_sides_of_what_fits_with_a_bank(r, n, k):
+    from thunderworld_b200 import ops
+    codes, scales = weights(n, k, 5)
+    bank, w1 = bank_of(n, k, .3, 6)
+    x, factor = rows_of(r, k, 7), torch.tensor(1e-3, device='cuda')
+    check(ops.fp4_matvec(x, codes, scales, factor, **bank), x, decoded(codes, scales) + w1, factor)
+
+
+def test_one_launch_for_all_rows_that_fit():
+    """The host's choice, as its description states it: the launches of a call by rows, K and bank."""
+    from thunderworld_b200 import _lib
+    launches = _lib.load().tw_matvec_launches
+    for k, fit, fit_bank in ((128, 32, 32), (4096, 32, 32), (14336, 32, 32), (16384, 29, 28), (24576, 21, 20), (32768, 16, 15)):
+        for bank, most in ((0, fit), (1, fit_bank)):
+            for rows in range(1, 33):
+                assert launches(rows, k, bank) == -(-rows // most), (rows, k, bank)
+    assert launches(0, 128, 0) == 0 and launches(33, 128, 0) == 0 and launches(1, 40, 0) == 0 and launches(1, 32800, 0) == 0

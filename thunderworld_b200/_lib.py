@@ -126,6 +126,7 @@ def load():
     lib.tw_gate_residual_norm.restype = _i
     lib.tw_capture_id.argtypes = [_vp]; lib.tw_capture_id.restype = ctypes.c_ulonglong
     lib.tw_matvec.argtypes = [ctypes.POINTER(MatvecArgs), _vp]; lib.tw_matvec.restype = _i
+    lib.tw_matvec_launches.argtypes = [_i] * 3; lib.tw_matvec_launches.restype = _i
     lib.tw_paged_attention_workspace.argtypes = [_i] * 4 + [_ll]; lib.tw_paged_attention_workspace.restype = ctypes.c_size_t
     lib.tw_paged_attention.argtypes = [ctypes.POINTER(PagedAttentionArgs), _vp]; lib.tw_paged_attention.restype = _i
     for name, count in (('append', 2), ('fork', 1), ('compact', 1)):
@@ -153,6 +154,6 @@ EXPORTS = ('tw_status', 'tw_abi_version', 'tw_quantize_workspace', 'tw_quantize'
            'tw_quantize_static_max_tiles', 'tw_swizzle_scales', 'tw_activation_rank', 'tw_selftest_bounded_wait',
            'tw_workspace', 'tw_fused', 'tw_fused_tile_n', 'tw_pack_rows', 'tw_select_tiles', 'tw_attention',
            'tw_attention_workspace', 'tw_activate', 'tw_rms_norm', 'tw_rms_norm_heads', 'tw_rope_heads', 'tw_gate_residual',
-           'tw_gate_residual_norm', 'tw_capture_id', 'tw_matvec',
+           'tw_gate_residual_norm', 'tw_capture_id', 'tw_matvec', 'tw_matvec_launches',
            'tw_paged_attention_workspace', 'tw_paged_attention', 'tw_cache_append_workspace', 'tw_cache_append', 'tw_cache_fork_workspace',
            'tw_cache_fork', 'tw_cache_free', 'tw_cache_compact_workspace', 'tw_cache_compact')

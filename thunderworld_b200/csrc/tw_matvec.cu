@@ -503,9 +503,24 @@ int launch(Params p, cudaStream_t stream) {
   return e == cudaSuccess ? TW_OK : TW_ERR_LAUNCH;
 }
 
+// Rows of each launch: the fewest even shares of the rows that fit a cluster of 8, since each reads all weights; at most 29 rows of a K of
+// 16384, 21 of 24576, 16 of 32768; with a bank 28, 20, 15. (20 x 4096 x 16384 48.6 us as two halves, 41.8 at once; 21 x 6144 x 24576
+// 86.1, 77.7; 17 with a quarter repaired 105.3, 90.5.)
+int rows_at_once(int rows, int kb, bool bank) {
+  int passes = 1, step = rows;
+  while (step > 1 && smem_bytes(step, kb, kb < 8 ? kb : 8, bank ? MAX_ROUNDS : 0) > MOST_SMEM) { ++passes; step = (rows + passes - 1) / passes; }
+  return step;
+}
+
 bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
 
 }  // namespace
+
+extern "C" int tw_matvec_launches(int rows, int k, int bank) {
+  if (rows <= 0 || rows > 32 || k <= 0 || k % 32 || k > 32768) return 0;
+  const int step = rows_at_once(rows, (k + 127) / 128, bank != 0);
+  return (rows + step - 1) / step;
+}
 
 extern "C" int tw_matvec(const TwMatvecArgs* a, void* stream) {
   if (!a || !a->x || !a->codes || !a->scales || !a->factor || !a->out || a->rows <= 0 || a->n <= 0 || a->k <= 0) return TW_ERR_ARGUMENT;
@@ -525,10 +540,7 @@ extern "C" int tw_matvec(const TwMatvecArgs* a, void* stream) {
   p.wr = a->wr; p.wrs = a->wrs; p.off = a->off; p.wi = a->wi; p.wloc = a->wloc; p.out = a->out;
   p.rows = a->rows; p.n = a->n; p.k = a->k; p.kb = (a->k + 127) / 128; p.nb = (a->n + 127) / 128;
   p.slots = a->slots; p.entries = a->entries; p.shared = a->shared; p.dense = a->dense; p.out_f32 = a->out_f32;
-  // 32 rows at a time, or what fits a cluster of 8: 16 rows of a K above 14336, 8 with a bank and a K above 31744
-  int most = 32;
-  while (most > 8 && smem_bytes(most, p.kb, p.kb < 8 ? p.kb : 8, bank ? MAX_ROUNDS : 0) > MOST_SMEM) most /= 2;
-  const int passes = (a->rows + most - 1) / most, step = (a->rows + passes - 1) / passes;
+  const int step = rows_at_once(a->rows, p.kb, bank);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   for (int row = 0; row < a->rows; row += step) {
     p.rows = a->rows - row < step ? a->rows - row : step;

@@ -240,7 +240,7 @@ def fp4_matvec(x, codes, scales, factor, *, prescale=None, bias=None, wr=None, w
     (wr [slots, 128, 64], wrs [slots, 128, 8]; wi, off, wloc, shared, dense as in fused_gemm), sums of 32 bits, one rounding.
     factor: float32 scalar tensor; prescale float32 [K]; bias bf16 [N]; out_dtype bfloat16 or float32; out shares no memory with x. Any
     N, K a multiple of 32 up to 32768; with a bank both multiples of 128. One launch; where the rows' part of K does not fit an SM's
-    shared memory (more than 16 rows of a K above 14336, with a bank more than 8 of a K above 31744) two to four, a share of the rows each."""
+    shared memory (more than 29 rows of a K of 16384, 21 of 24576, 16 of 32768, with a bank 28, 20, 15) two or three, a share of the rows each."""
     if x.ndim < 1 or x.dtype is not torch.bfloat16 or not x.is_cuda:
         raise ValueError('expected CUDA BF16 rows [..., K]')
     if codes.ndim != 2 or codes.dtype is not torch.uint8 or not codes.is_contiguous():
