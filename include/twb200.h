@@ -132,7 +132,8 @@ int tw_fused_tile_n(int n);
 
 /* ---- products of a few rows ------------------------------------------------------------------
  * out[r, n] = rnd( factor * sum_k bf16(x[r, k] * prescale[k]) * W[n, k] + bias[n] ), 1 <= r <= 32: the packed weights of
- * tw_fused for a token at a time. x stays bf16 (no activation planes), sums are 32 bits wide, one rounding at the end.
+ * tw_fused for a token at a time. x stays bf16 (no activation planes), sums are 32 bits wide, one rounding at the end. Of a
+ * row, values below 2^-29 of the largest are held to within 2^-39 of the largest, all others exactly.
  * W[n, k] = code * scale (scale per 16 k), plus the bank's tile where (n / 128, k / 128) has one; bank layout, CSR, shared and
  * dense as in TwRepairIO, every (n / 128, k / 128) at most once. Any n; k % 32 == 0, k <= 32768; with a bank n and k multiples of 128.
  * Entries of off / wi / wloc that lead outside wi, K or the bank are left out. out must not overlap x. */
@@ -203,7 +204,8 @@ int tw_attention(const TwAttentionArgs* args, void* stream);
 /* ---- attention of one token over a paged cache -------------------------------------------------
  * out[b, h] = sum_t softmax_t(scale * q[b, h] . k_t) v_t over the tokens t < lengths[s] of slot s = slots[b] (b when slots is
  * NULL), k_t = k_pages[table[s, t / page], h / (hq / hk), t % page] (times k_scale[h / (hq / hk)]), v_t alike. An empty
- * sequence gives zeros and lse = -inf. What lies behind a sequence's end in its last page is not used, whatever it is.
+ * sequence gives zeros and lse = -inf. Sums are 32 bits wide; a probability is rounded before it meets the values, by 2^-16 of itself
+ * with bf16 pages, by 2^-12 with E4M3 ones. What lies behind a sequence's end in its last page is not used, whatever it is.
  * Pages: [pages, hk, page, dim], rows contiguous, bf16 or (fp8) E4M3; page a power of two; dim 64 or 128; any hq / hk.
  * A slot, length or table entry that leads outside is left out (its tokens do not count) and reported in *status. Scratch needs no
  * initialisation; calls that may overlap need scratch of their own, and must not overlap a call that changes the cache.

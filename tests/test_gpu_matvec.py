@@ -372,3 +372,23 @@ def test_one_launch_for_all_rows_that_fit():
             for rows in range(1, 33):
                 assert launches(rows, k, bank) == -(-rows // most), (rows, k, bank)
     assert launches(0, 128, 0) == 0 and launches(33, 128, 0) == 0 and launches(1, 40, 0) == 0 and launches(1, 32800, 0) == 0
+
+
+@gpu
+@pytest.mark.parametrize('power', [24, 28, 33, 40, 60])
+@pytest.mark.parametrize('r', [1, 9])
+def test_values_below_what_is_held_beside_an_outlier(power, r):
+    """As above with larger outliers: what is not held exactly, values below 2^-29 of the largest, is off by 2^-39 of the largest at most,
+    in the CTA that has the outlier's part of K."""
+    from thunderworld_b200 import ops
+    codes, scales = weights(40, 512, 1, high=4.)
+    scales.view(torch.uint8)[:, 0] = 0
+    x = rows_of(r, 512, 3)
+    x[:, 5] = 2. ** power
+    factor = torch.tensor(1., device='cuda')
+    w = decoded(codes, scales)
+    y = ops.fp4_matvec(x, codes, scales, factor, out_dtype=torch.float32).double()
+    x[:, 5] = 0
+    want, size = x.double() @ w.T, x.double().abs() @ w.abs().T
+    bound = 2. ** -24 * want.abs() + (512 / 128 + 32) * 2. ** -22 * size + 2. ** (power - 39) * w.abs().sum(1)
+    assert ((y - want).abs() <= bound).all()

@@ -5,7 +5,8 @@
 // exact in f16 (2^-10 ... 2688), and the tensor cores multiply f16 exactly into 32-bit sums: m16n8k16 with 16 weight rows as A and
 // up to 8 rows of x as B. x is bf16, whose exponents f16 does not have: every CTA scales its part of a row by a power of two
 // that brings the largest value to [2^14, 2^15). That is exact but for values 2^29 below the largest, whose last
-// bits, 2^-39 of the largest, are rounded away, far below the 2^-24 of the sums; the sums are scaled back.
+// bits are rounded away, at most 2^-39 of the largest each: far below the 2^-24 of the sums, unless all weights that the largest meets
+// are zero (a second f16 value for the rest would double the products). The sums are scaled back.
 //
 // What bounds it is the read of the weights, 9/16 byte each, once. A lane loads 16 bytes of codes (32 of k) of two rows and the two
 // scales of each; four lanes cover a K128 block of a row, and each lane's 32 k-values may sit in any k-slot of the

@@ -237,7 +237,8 @@ def fp4_matvec(x, codes, scales, factor, *, prescale=None, bias=None, wr=None, w
     """Product of a few rows (at most 32) with packed NVFP4 weights, for a token at a time: x bf16 [..., K] stays bf16.
 
     y = factor * (bf16(x * prescale) @ W.T) + bias, W = codes [N, K/2] x E4M3 scales [N, K/16] plus the W1 tiles of a bank
-    (wr [slots, 128, 64], wrs [slots, 128, 8]; wi, off, wloc, shared, dense as in fused_gemm), sums of 32 bits, one rounding.
+    (wr [slots, 128, 64], wrs [slots, 128, 8]; wi, off, wloc, shared, dense as in fused_gemm), sums of 32 bits, one rounding. Of a row,
+    values below 2^-29 of the largest are held to within 2^-39 of the largest, all others exactly.
     factor: float32 scalar tensor; prescale float32 [K]; bias bf16 [N]; out_dtype bfloat16 or float32; out shares no memory with x. Any
     N, K a multiple of 32 up to 32768; with a bank both multiples of 128. One launch; where the rows' part of K does not fit an SM's
     shared memory (more than 29 rows of a K of 16384, 21 of 24576, 16 of 32768, with a bank 28, 20, 15) two or three, a share of the rows each."""
@@ -397,7 +398,8 @@ def paged_attention(q, k_pages, v_pages, table, lengths, *, slots=None, scale=No
     Pages [pages, kv_heads, page, dim] in bf16 or float8_e4m3fn (times k_scale / v_scale [kv_heads]), page a power of two, dim 64 or
     128; table int32 [sequences, pages per sequence], lengths int32 [sequences], slots int32 [batch], all read on the device:
     no host synchronisation. scale defaults to dim ** -0.5. Returns bf16 [batch, heads, dim], with return_lse also the float32
-    natural log of each softmax's sum (-inf and zeros for an empty sequence). Sums are 32 bits wide. Slots, lengths and table entries
+    natural log of each softmax's sum (-inf and zeros for an empty sequence). Sums are 32 bits wide; probabilities are
+    rounded before they meet the values, by 2^-16 of themselves with bf16 pages, 2^-12 with E4M3 ones. Slots, lengths and table entries
     that lead outside are left out and reported by device_status(). Can be captured, except for a device's first paged call."""
     pages, hk, page, dim, fp8, ks, vs = _check_pages(k_pages, v_pages)
     dev = k_pages.device
