@@ -105,7 +105,8 @@ _workspaces = {}
 def _workspace(device, nbytes, key):
     ws = _workspaces.get((device, key))
     if ws is None or ws.numel() < nbytes:
-        ws = torch.zeros(max(nbytes, 256), device=device, dtype=torch.uint8)
+        with torch.inference_mode(False):                 # reset_device_status writes to it outside of that mode as well
+            ws = torch.zeros(max(nbytes, 256), device=device, dtype=torch.uint8)
         _workspaces[(device, key)] = ws
     return ws
 
