@@ -61,7 +61,7 @@ class PagedCache:
         return ops.cache_compact_(*self._pools, *self._tables)
 
     def check(self):
-        """Raise if any paged operator on this device left something out since the status was last reset (synchronises)."""
+        """Raise if any paged operator on this device, on whatever stream, left something out since the status was last reset (waits for it)."""
         status = ops.device_status(self.k_pages.device)
         if status:
             raise RuntimeError(load().tw_status(status).decode())

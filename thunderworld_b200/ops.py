@@ -559,12 +559,13 @@ STATUS_KEYS = {'g': 0, 'a': 0, 'q': 8, 'c': 0}   # workspace -> byte offset of i
 
 
 def device_status(device=None):
-    """Worst status word any kernel of this device wrote on a bounded-wait timeout (0 = none); synchronises.
+    """Worst status word any kernel of this device wrote on a bounded-wait timeout (0 = none); waits for all streams of the device.
     Covers the fused GEMM, the attention kernel and the single-pass quantizer's grid barrier: each writes into its own workspace;
     and what the operators of the paged cache found and left out (an entry outside the cache, a full pool)."""
     dev = torch.device('cuda', torch.cuda.current_device()) if device is None else torch.device(device)
     if dev.index is None:
         dev = torch.device('cuda', torch.cuda.current_device())
+    torch.cuda.synchronize(dev)
     worst = 0
     for key, offset in STATUS_KEYS.items():
         ws = _workspaces.get((dev, key))
@@ -574,14 +575,16 @@ def device_status(device=None):
 
 
 def reset_device_status(device=None):
-    """Clear the status words (after a reported timeout has been handled)."""
+    """Clear the status words (after a reported timeout has been handled); waits for all streams of the device, before and after."""
     dev = torch.device('cuda', torch.cuda.current_device()) if device is None else torch.device(device)
     if dev.index is None:
         dev = torch.device('cuda', torch.cuda.current_device())
+    torch.cuda.synchronize(dev)
     for key, offset in STATUS_KEYS.items():
         ws = _workspaces.get((dev, key))
         if ws is not None:
             ws[offset:offset + 4].zero_()
+    torch.cuda.synchronize(dev)
 
 
 # ---- pointwise producers with fused tensor factor -----------------------------------------------
