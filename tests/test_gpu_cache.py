@@ -464,3 +464,16 @@ def test_compact_leaves_a_bad_entry_as_it_is(entry):
     assert ops.device_status() == 11
     ops.reset_device_status()
     model.same(cache)
+
+
+@gpu
+def test_offsets_that_hold_nothing_are_refused():
+    """cu has one offset at least: an empty one is a mistake, not a call with nothing to do."""
+    cache = make(6, 4, 2, 64, False)
+    x = torch.zeros(2, 2, 64, device='cuda', dtype=torch.bfloat16)
+    for slots in (None, i32([])):
+        with pytest.raises(ValueError, match='one offset more'):
+            cache.append(x, x, slots, i32([]))
+    cache.append(x, x, None, i32([0]))
+    cache.append(x, x, i32([]), i32([2]))
+    assert not cache.lengths.any()

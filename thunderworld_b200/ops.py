@@ -485,7 +485,7 @@ def cache_append_(k, v, k_pages, v_pages, table, lengths, refs, *, slots=None, c
     _check_scales(dev, hk, k_scale, v_scale, fp8)
     rows = shape[0]
     batch = slots.numel() if slots is not None else (cu.numel() - 1 if cu is not None else rows)
-    if (cu is None and batch != rows) or (cu is not None and cu.numel() != batch + 1):
+    if (cu is None and batch != rows) or (cu is not None and (cu.numel() != batch + 1 or batch < 0)):
         raise ValueError('one row per slot, or cu with one offset more than there are slots, is required')
     if slots is None and batch > sequences:
         raise ValueError('more entries than sequences')
