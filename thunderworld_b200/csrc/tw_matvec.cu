@@ -21,8 +21,8 @@
 // next 128 rows' products. No workspace, no atomics on sums: the order is fixed.
 //
 // Measured (B200, weights from HBM, graph replay; bytes of the weights over time): 1 x 24576 x 6144 23.3 us (3.7 TB/s), 1 x 12288 x
-// 4096 12.6 us, 8 x 16384 x 4096 16.9 us, 32 x 16384 x 4096 36.1 us, 5 x 6144 x 24576 with a quarter repaired 35.9 us (3.0 TB/s), 1 x
-// 2048 x 2048 4.7 us. What bounds it: of the 23 us of 24576 x 6144, some 7 are start (launch, instructions from L2, x to f16)
+// 4096 12.6 us, 8 x 16384 x 4096 16.8 us, 16 and 32 rows 21.9 and 35.8 us (a prescale adds 0.5, 1.2, 1.2 and 2.6 us), 5 x 6144 x 24576 with a
+// quarter repaired 36 us (3.0 TB/s), 1 x 2048 x 2048 4.9 us. What bounds it: of the 23 us of 24576 x 6144, some 7 are start (launch, instructions from L2, x to f16)
 // and join (cluster barriers, cold code); then the decoding and the stream of the weights hide each other in part only: without the
 // decoding, or without the copies, it takes 2 us and 1 us less, without both products and decoding 5 us. More warps (24 or 32
 // per SM), a third quad on the way, chains of products and x loaded ahead change nothing, the next block's codes ahead cost 1 us.

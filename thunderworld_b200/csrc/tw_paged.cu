@@ -22,11 +22,12 @@
 // and read as zeros, whatever lies there.
 //
 // Measured (B200, pages from HBM, graph replay; both launches; 32 heads on 8 or 4, dim 128): 24 sequences of 0 ... 8192 tokens in pages
-// of 16 69.2 us (5.4 TB/s of keys and values); 48 of up to 16384 with E4M3 pages 67 us (4.2 TB/s); one of 100000 tokens 76 us
-// (5.4 TB/s); 32 of 4096 41.1 us (4.5 TB/s); one of 3840 tokens 13.9 us; 32 of up to 8192 with 32 heads on 2 30.3 us (3.1 TB/s). The
-// large bf16 cases are held by memory (12 warps per SM wait for it, long scoreboard the first stall); with E4M3 pages the instructions
-// per byte double (1.6 issued per cycle and SM); small calls by their chain of start, lengths, table, pages, warps' join, second
-// launch. Three times as many smaller runs, an earlier launch of the join and branch hints changed nothing.
+// of 16 69.7 us (5.4 TB/s of keys and values), of 4 95 us, of 1 107 us; 48 of up to 16384 with E4M3 pages 67.7 us (4.2 TB/s); one of 100000 tokens
+// 76.7 us (5.3 TB/s); 32 of 4096 41.7 us (4.5 TB/s); one of 3840 tokens 13.7 us; 32 of up to 8192 with 32 heads on 2 30.5 us (3.1 TB/s), E4M3 27.3 us;
+// 16 of up to 4096 with 32 heads on 32 71.8 us (5.4 TB/s). The large bf16 cases are held by memory (12 warps per SM wait for it, long scoreboard the
+// first stall); E4M3 ones by latency: half the bytes per tile for the same chain of products, maxima and exponentials, 1.65 instructions per
+// cycle and SM of four; wide groups of 128 channels by two warps per scheduler; small calls by their chain of start, lengths, table, pages,
+// warps' join, second launch. The narrow kernels of 128 channels spill 92 and 114 bytes at 168 registers. Three times as many smaller runs, an earlier launch of the join and branch hints changed nothing.
 #include <atomic>
 #include "tw_common.cuh"
 #include "../../include/twb200.h"

@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(256) gate_residual_kernel(uint4* __restrict__ 
 // x' = bf16(residual_scale * x + gate * z);  h = bf16(x' * rsqrt(mean(x'^2) + eps) [* weight] [* (1 + scale) + shift]).
 // A CTA owns a row at a time; a row of x and y is read once, x' stays in registers between the two norms, so a pass
 // moves 8 bytes per element where gate_residual and rms_norm one after the other move 10 (HBM-bound: at 7680 x 4096 with
-// modulation and factor 47.8 us, 5.3 TB/s; the two kernels 70.1 us). x' is rounded before it is
+// modulation and factor 48 us, 5.2 TB/s; the two kernels 70.1 us; with POST and modulation 55 us, two reductions per row one behind the other). x' is rounded before it is
 // squared, because the next block reads the rounded stream; z is not rounded on its own. The sums of squares are
 // held in 32 bits and taken in rms_norm_kernel's order, so that without POST and with residual_scale = 1 the bits
 // are those of the two kernels.
