@@ -559,7 +559,8 @@ STATUS_KEYS = {'g': 0, 'a': 0, 'q': 8, 'c': 0}   # workspace -> byte offset of i
 
 
 def device_status(device=None):
-    """Worst status word any kernel of this device wrote on a bounded-wait timeout (0 = none); waits for all streams of the device.
+    """Worst status word any kernel of this device wrote on a bounded-wait timeout (0 = none); waits for all streams of the device,
+    so not while one of them is being captured.
     Covers the fused GEMM, the attention kernel and the single-pass quantizer's grid barrier: each writes into its own workspace;
     and what the operators of the paged cache found and left out (an entry outside the cache, a full pool)."""
     dev = torch.device('cuda', torch.cuda.current_device()) if device is None else torch.device(device)
